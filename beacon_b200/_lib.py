@@ -43,6 +43,9 @@ EXPORTS = (
     "beacon_layernorm_adjoint_fwd", "beacon_layernorm_adjoint_bwd",
     "beacon_swiglu_adjoint_fwd", "beacon_swiglu_adjoint_bwd", "beacon_swiglu_workspace_size",
     "beacon_llama_block_fwd", "beacon_llama_block_workspace_size", "beacon_llama_block_fwd_folded",
+    "beacon_rope_table", "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd",
+    "beacon_qk_norm_rope_bwd_workspace_size", "beacon_qk_norm_rope_append",
+    "beacon_paged_attention_fwd", "beacon_paged_attention_workspace_size",
     "beacon_residual_add_fwd", "beacon_residual_add_bwd", "beacon_cast",
     "beacon_embedding_lookup_fwd", "beacon_embedding_lookup_bwd", "beacon_dropout_fwd", "beacon_dropout_bwd",
     "beacon_arena_create", "beacon_arena_destroy", "beacon_arena_base", "beacon_arena_size", "beacon_launch",
@@ -132,6 +135,18 @@ def lib():
     _sig(L, "beacon_llama_block_fwd", _int, [_vp] * 9 + [_i64] * 7 + [ctypes.c_float, _int, _vp, _sz, _vp])
     _sig(L, "beacon_llama_block_workspace_size", _sz, [_i64] * 7 + [_int])
     _sig(L, "beacon_llama_block_fwd_folded", _int, [_vp] * 7 + [_i64] * 7 + [ctypes.c_float, _int, _vp, _sz, _vp])
+    _sig(L, "beacon_rope_table", _int, [_vp, _i64, _i64, ctypes.c_double, _vp])
+    _sig(L, "beacon_qk_norm_rope_fwd", _int,
+         [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64, _vp] + [_i64] * 6 + [_int, ctypes.c_float, _int, _vp])
+    _sig(L, "beacon_qk_norm_rope_bwd", _int,
+         [_vp, _i64] + [_vp] * 6 + [_i64] + [_vp] * 3 + [_i64, _vp] + [_i64] * 6 +
+         [_int, ctypes.c_float, _int, _vp, _sz, _vp])
+    _sig(L, "beacon_qk_norm_rope_bwd_workspace_size", _sz, [_i64])
+    _sig(L, "beacon_qk_norm_rope_append", _int,
+         [_vp] * 4 + [_i64] + [_vp] * 3 + [_i64] + [_vp] * 4 + [_i64] * 13 + [_int, ctypes.c_float, _int, _vp])
+    _sig(L, "beacon_paged_attention_fwd", _int,
+         [_vp] * 3 + [_i64] + [_vp] * 5 + [_i64] * 13 + [_int, _int, _vp, _sz, _vp])
+    _sig(L, "beacon_paged_attention_workspace_size", _sz, [_i64, _int])
     _sig(L, "beacon_residual_add_fwd", _int, [_vp, _vp, _vp, _i64, _int, _vp])
     _sig(L, "beacon_residual_add_bwd", _int, [_vp, _vp, _vp, _i64, _int, _vp])
     _sig(L, "beacon_cast", _int, [_vp, _vp, _i64, _int, _vp])

@@ -16,6 +16,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -27,6 +28,9 @@
 #include "elementwise.cuh"
 #include "gemm.cuh"
 #include "gemm_fp8.cuh"
+#include "paged.cuh"
+#include "paged_tc.cuh"
+#include "rope.cuh"
 #include "sm100.cuh"
 
 using namespace beacon;
@@ -1551,5 +1555,6 @@ extern "C" int beacon_rmsnorm_adjoint_bwd_noalloc(void* dx, void* dweight, const
 
 #include "abi_attention.inc"
 #include "abi_swiglu.inc"
+#include "abi_paged.inc"
 #include "abi_block.inc"
 #include "abi_arena.inc"

@@ -1,0 +1,396 @@
+// paged.cuh -- attention of new tokens over a paged key/value cache: work distribution, the exact
+// SIMT kernel, and the kernel that joins split work.
+//
+// Sequence s brings q_len = cu_q[s+1] - cu_q[s] new tokens and kv = kv_lens[s] cached ones, the new
+// ones last.  New token i sits at p = kv - q_len + i and sees keys j <= p (causal) or j < kv:
+//   out = softmax(q k^T / sqrt(D)) v, lse = log sum exp; no key visible: out = 0, lse = -inf.
+// For one KV head the rows are (token, query head of the group), token-major: R = q_len * g.
+//
+// Work: an item is `rpi` consecutive rows of one (sequence, KV head); its length is the number of
+// 128- (or 64-) key tiles its last row sees, at least one.  All items laid end to end (sequence, KV
+// head, item, tile) are cut into gridDim.x equal runs of tiles, one per CTA, so that one long
+// context fills the GPU as well as many short ones and the SMs finish together.  A run's first and
+// last item may be partial: their unnormalised rows (O, m, l) go to two workspace slots of the CTA
+// and k_paged_join adds them up in tile order, so results do not depend on timing.  Every CTA finds
+// its run itself from cu_q and kv_lens (one warp, 32 sequences per step): no plan, no host copy.
+#pragma once
+
+#include "rope.cuh"
+#include "sm100.cuh"
+
+namespace beacon {
+
+struct PagedParams {
+  PagedSeqs pg;
+  int Hq, Hkv, D, g;         // g = Hq / Hkv
+  int causal;
+  int rpi;                   // rows per item
+  float scale;               // 1 / sqrt(D)
+  long long q_stride;        // elements between token rows of q
+  long long tokens;
+  void* out;                 // [tokens, Hq, D]
+  float* lse;                // [tokens, Hq] or null
+  int4* heads;               // [gridDim.x] the split item that begins in this CTA's run (paged_head)
+  float* part_o;             // [2 * gridDim.x, rpi, D]
+  float2* part_ml;           // [2 * gridDim.x, rpi] (running maximum, in log2 units; sum)
+};
+
+enum : unsigned int {
+  kSitePagedLens = 0x611,  // cu_q or kv_lens reach past the query rows or the page table
+  kSitePagedPage = 0x612,  // a page index outside the cache
+};
+
+// One contiguous piece of an item: tiles [a, b) of its n.
+struct PagedItem {
+  int seq, kvh, row0;  // first row within the sequence's R
+  int q0, q_len, kv;   // first token, new tokens, cached tokens of the sequence
+  int a, b, n;
+};
+
+// Tiles of item i of a sequence.
+__device__ __forceinline__ int paged_tiles(int i, int rpi, int g, int q_len, int kv, int causal, int kt) {
+  const long long rows = (long long)q_len * g;
+  const long long last = (min((long long)(i + 1) * rpi, rows) - 1) / g;
+  const long long keys = causal ? max(0LL, (long long)kv - q_len + last + 1) : (long long)kv;
+  return max(1, (int)((keys + kt - 1) / kt));
+}
+// First token, new tokens and cached tokens of sequence s, held inside the tensors that they index.
+__device__ __forceinline__ void paged_lens(const PagedParams& p, int s, int& q0, int& q_len, int& kv) {
+  q0 = __ldg(p.pg.cu_q + s);
+  q_len = max(0, __ldg(p.pg.cu_q + s + 1) - q0);
+  kv = max(0, __ldg(p.pg.kv_lens + s));
+  const long long most = (long long)p.pg.max_pages * p.pg.page_size;
+  if (q0 < 0 || (long long)q0 + q_len > p.tokens || kv > most) {
+    record_fault(kFaultIndex, kSitePagedLens);
+    q0 = max(q0, 0);
+    q_len = (int)max(0LL, min((long long)q_len, p.tokens - q0));
+    kv = (int)min((long long)kv, most);
+  }
+}
+__device__ __forceinline__ long long paged_seq_work(const PagedParams& p, int s, int kt) {
+  if (s >= p.pg.seqs) return 0;
+  int q0, q_len, kv;
+  paged_lens(p, s, q0, q_len, kv);
+  const int n = (int)(((long long)q_len * p.g + p.rpi - 1) / p.rpi);
+  if (!p.causal) return (long long)n * paged_tiles(0, p.rpi, p.g, q_len, kv, 0, kt);
+  long long w = 0;
+  for (int i = 0; i < n; ++i) w += paged_tiles(i, p.rpi, p.g, q_len, kv, 1, kt);
+  return w;
+}
+
+// A CTA's run of tiles, walked item by item by one warp (every lane holds the same state).
+struct PagedWalk {
+  long long left, chunk;  // tiles left in the run; tiles per run
+  int seq, kvh, item, tile;
+  int q0, q_len, kv, items;
+
+  __device__ __forceinline__ void start(const PagedParams& p, int kt) {
+    const int lane = (int)lane_id();
+    long long total = 0;
+    const long long w0 = paged_seq_work(p, lane, kt);
+    for (int s = lane; s < p.pg.seqs; s += 32) total += (s == lane) ? w0 : paged_seq_work(p, s, kt);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= p.Hkv;
+    chunk = max(1LL, (total + gridDim.x - 1) / gridDim.x);
+    long long at = min((long long)blockIdx.x * chunk, total);
+    left = min(chunk, total - at);
+    if (left <= 0) return;
+    for (int s0 = 0; s0 < p.pg.seqs; s0 += 32) {
+      const long long w = (s0 == 0 ? w0 : paged_seq_work(p, s0 + lane, kt)) * p.Hkv;
+      long long end = w;  // inclusive prefix sum
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, at < end);
+      if (hit != 0) {
+        const int l = __ffs(hit) - 1;
+        const long long seq_work = __shfl_sync(0xffffffffu, w, l);
+        at -= __shfl_sync(0xffffffffu, end, l) - seq_work;
+        seq = s0 + l;
+        enter(p);
+        const long long per_head = seq_work / p.Hkv;
+        kvh = (int)(at / per_head);
+        at -= kvh * per_head;
+        item = 0;
+        for (int n = paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt); at >= n;
+             n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt)) {
+          at -= n;
+          ++item;
+        }
+        tile = (int)at;
+        return;
+      }
+      at -= __shfl_sync(0xffffffffu, end, 31);
+    }
+    left = 0;
+  }
+  __device__ __forceinline__ void enter(const PagedParams& p) {
+    paged_lens(p, seq, q0, q_len, kv);
+    items = (int)(((long long)q_len * p.g + p.rpi - 1) / p.rpi);
+  }
+  // The next piece; false at the end of the run.
+  __device__ __forceinline__ bool next(const PagedParams& p, int kt, PagedItem& x) {
+    if (left <= 0) return false;
+    x.seq = seq;
+    x.kvh = kvh;
+    x.row0 = item * p.rpi;
+    x.q0 = q0;
+    x.q_len = q_len;
+    x.kv = kv;
+    x.n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt);
+    x.a = tile;
+    x.b = (int)min((long long)x.n, tile + left);
+    left -= x.b - x.a;
+    tile = 0;
+    if (++item >= items) {
+      item = 0;
+      if (++kvh >= p.Hkv) {
+        kvh = 0;
+        if (left > 0) {
+          do {
+            ++seq;
+            enter(p);
+          } while (items == 0 && seq + 1 < p.pg.seqs);  // work is left, so a sequence with tokens follows
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// The split item that begins in a CTA's run, for the join: x = seq, y = KV head, z = item, w = the
+// number of following CTAs that hold the rest of it (0: none begins here).
+__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x, long long chunk) {
+  return make_int4(x.seq, x.kvh, x.row0 / p.rpi, (int)((x.n - x.b + chunk - 1) / chunk));
+}
+// Workspace slot of a partial piece: a piece that continues an item is the run's first.
+__device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
+
+// Keys that row r (of R) of a piece sees.
+__device__ __forceinline__ int paged_limit(const PagedParams& p, const PagedItem& x, int r) {
+  return p.causal ? max(0, x.kv - x.q_len + r / p.g + 1) : x.kv;
+}
+
+// Element offset of key j of a sequence for a KV head, or -1 when its page is not in the cache.
+__device__ __forceinline__ long long paged_key(const PagedSeqs& g, int seq, int kvh, int j) {
+  const int pi = j / g.page_size;
+  const int page = __ldg(g.page_table + (long long)seq * g.table_stride + pi);
+  if (page < 0 || page >= g.num_pages) {
+    record_fault(kFaultIndex, kSitePagedPage);
+    return -1;
+  }
+  return (long long)page * g.page_stride + (long long)kvh * g.head_stride +
+         (long long)(j - pi * g.page_size) * g.token_stride;
+}
+
+// ---------------------------------------------------------------------------
+// Exact path: float32 (and bf16 caches whose pages TMA cannot describe), fp32 FFMA, expf.
+// 256 threads; tiles of BM rows x 64 keys; Q, K, V and P in shared memory as fp32, each thread
+// BM/16 rows x 4 keys of S and BM/16 rows x D/16 columns of O in registers.
+// ---------------------------------------------------------------------------
+constexpr int kPagedSimtKt = 64;
+template <int D, int BM>
+constexpr size_t paged_simt_smem() {
+  return sizeof(float) * ((size_t)(BM + 2 * kPagedSimtKt) * (D + 4) + (size_t)BM * (kPagedSimtKt + 4) + 2 * BM);
+}
+
+template <typename T, int D, int BM>
+__global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q, const T* __restrict__ kc,
+                                                         const T* __restrict__ vc, const PagedParams p) {
+  constexpr int KT = kPagedSimtKt, LD = D + 4, LP = KT + 4, RT = BM / 16, CT = D / 16;
+  extern __shared__ __align__(16) float fsm[];
+  float* sq = fsm;
+  float* sk = sq + BM * LD;
+  float* sv = sk + KT * LD;
+  float* sp = sv + KT * LD;
+  float* s_m = sp + BM * LP;
+  float* s_l = s_m + BM;
+  __shared__ PagedItem item;
+  __shared__ int more;
+  const int tid = (int)threadIdx.x;
+  const int ty = tid >> 4, tx = tid & 15;  // S rows ty + 16 i, keys tx + 16 j; O columns tx + 16 c
+  PagedWalk walk;
+  if (warp_id() == 0) {
+    walk.start(p, KT);
+    if (tid == 0) p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
+  const int group = p.g;
+  for (;;) {
+    __syncthreads();
+    if (warp_id() == 0) {
+      PagedItem x;
+      const bool ok = walk.next(p, KT, x);
+      if (tid == 0) {
+        more = ok ? 1 : 0;
+        item = x;
+        if (ok && x.a == 0 && x.b < x.n) p.heads[blockIdx.x] = paged_head(p, x, walk.chunk);
+      }
+    }
+    __syncthreads();
+    if (!more) break;
+    const PagedItem x = item;
+    const int rows = min(p.rpi, x.q_len * group - x.row0);
+    for (int e = tid; e < BM * D; e += 256) {
+      const int r = e / D, d = e % D;
+      float v = 0.0f;
+      if (r < rows) {
+        const int fr = x.row0 + r;
+        v = ldf(q + (long long)(x.q0 + fr / group) * p.q_stride + ((long long)x.kvh * group + fr % group) * D + d);
+      }
+      sq[r * LD + d] = v * p.scale;
+    }
+    if (tid < BM) {
+      s_m[tid] = -INFINITY;
+      s_l[tid] = 0.0f;
+    }
+    float o[RT][CT] = {};
+    for (int j = x.a; j < x.b; ++j) {
+      const int k0 = j * KT;
+      __syncthreads();
+      for (int e = tid; e < KT * (D / 4); e += 256) {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
+        if (k0 + r < x.kv) {
+          const long long at = paged_key(p.pg, x.seq, x.kvh, k0 + r);
+          if (at >= 0) {
+            kf = make_float4(ldf(kc + at + d), ldf(kc + at + d + 1), ldf(kc + at + d + 2), ldf(kc + at + d + 3));
+            vf = make_float4(ldf(vc + at + d), ldf(vc + at + d + 1), ldf(vc + at + d + 2), ldf(vc + at + d + 3));
+          }
+        }
+        *reinterpret_cast<float4*>(sk + r * LD + d) = kf;
+        *reinterpret_cast<float4*>(sv + r * LD + d) = vf;
+      }
+      __syncthreads();
+      float s[RT][4] = {};
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 kf[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * LD + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float4 qf = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * LD + d);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[i][c] = fmaf(qf.x, kf[c].x, fmaf(qf.y, kf[c].y, fmaf(qf.z, kf[c].z, fmaf(qf.w, kf[c].w, s[i][c]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = ty + 16 * i;
+        const int limit = (r < rows ? paged_limit(p, x, x.row0 + r) : 0) - k0;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (tx + 16 * c >= limit) s[i][c] = -INFINITY;
+          mx = fmaxf(mx, s[i][c]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float m_old = s_m[r], m_new = fmaxf(m_old, mx);
+        const float base = m_new == -INFINITY ? 0.0f : m_new;  // a row that has seen no key yet
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float e = expf(s[i][c] - base);
+          sp[r * LP + tx + 16 * c] = e;
+          sum += e;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        const float alpha = expf(m_old - base);
+        __syncwarp();
+        if (tx == 0) {
+          s_m[r] = m_new;
+          s_l[r] = s_l[r] * alpha + sum;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[i][c] *= alpha;
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int kk = 0; kk < KT; ++kk) {
+        float vf[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) vf[c] = sv[kk * LD + tx + 16 * c];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float pf = sp[(ty + 16 * i) * LP + kk];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) o[i][c] = fmaf(pf, vf[c], o[i][c]);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = x.a == 0 && x.b == x.n;
+    const int slot = paged_slot(x);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty + 16 * i;
+      if (r >= rows) continue;
+      const float m = s_m[r], l = s_l[r];
+      if (whole) {
+        const int fr = x.row0 + r;
+        const long long at = (long long)(x.q0 + fr / group) * p.Hq + (long long)x.kvh * group + fr % group;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) stf((T*)p.out + at * D + tx + 16 * c, o[i][c] * inv);
+        if (tx == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
+      } else {
+        float* po = p.part_o + ((long long)slot * p.rpi + r) * D;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) po[tx + 16 * c] = o[i][c];
+        if (tx == 0) p.part_ml[(long long)slot * p.rpi + r] = make_float2(m * 1.4426950408889634f, l);
+      }
+    }
+  }
+}
+
+// Joins split items: CTA (c, y) merges rows y, y + gridDim.y, ... (a warp each) of the item that begins
+// in run c: its piece in slot 2c + 1 and the continuations in slots 2(c + 1), 2(c + 2), ... in order.
+// With M = max m: out = sum 2^(m - M) O / sum 2^(m - M) l.
+template <typename T>
+__global__ void __launch_bounds__(128) k_paged_join(const PagedParams p) {
+  const int c = (int)blockIdx.x, lane = (int)lane_id();
+  const int4 h = p.heads[c];
+  if (h.w == 0) return;
+  int q0, q_len, kv;
+  paged_lens(p, h.x, q0, q_len, kv);
+  const int row0 = h.z * p.rpi;
+  const int rows = min(p.rpi, q_len * p.g - row0);
+  for (int r = (int)(blockIdx.y * 4 + warp_id()); r < rows; r += 4 * (int)gridDim.y) {
+    float mx = -INFINITY;
+    for (int i = lane; i <= h.w; i += 32) {
+      const long long slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+      mx = fmaxf(mx, p.part_ml[slot * p.rpi + r].x);
+    }
+  #pragma unroll
+    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    float l = 0.0f, o[kRopeMaxDim / 32] = {};
+    for (int i = 0; i <= h.w; ++i) {
+      const long long slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+      const float2 ml = p.part_ml[slot * p.rpi + r];
+      if (ml.x == -INFINITY) continue;  // the piece saw no key of this row; its O was not written
+      const float wgt = exp2f(ml.x - base);
+      l = fmaf(ml.y, wgt, l);
+      const float* po = p.part_o + (slot * p.rpi + r) * p.D;
+#pragma unroll
+      for (int e = 0; e < kRopeMaxDim / 32; ++e)
+        if (lane + 32 * e < p.D) o[e] = fmaf(po[lane + 32 * e], wgt, o[e]);
+    }
+    const int fr = row0 + r;
+    const long long at = (long long)(q0 + fr / p.g) * p.Hq + (long long)h.y * p.g + fr % p.g;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < kRopeMaxDim / 32; ++e)
+      if (lane + 32 * e < p.D) stf((T*)p.out + at * p.D + lane + 32 * e, o[e] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[at] = l > 0.0f ? (base + log2f(l)) * 0.69314718055994531f : -INFINITY;
+  }
+}
+
+}  // namespace beacon

@@ -1,0 +1,549 @@
+// paged_tc.cuh -- attention of new tokens over a paged cache on tcgen05 tensor cores (bf16, head_dim
+// 64 or 128, pages of a multiple of 8 tokens; definitions and work distribution in paged.cuh).
+//
+// One CTA per SM walks its run of key tiles.  An item is a pair of 128-row query tiles (A, B) of one
+// (sequence, KV head); a tile's rows are tpt = floor(128 / g) tokens x g heads of the group, fetched by
+// one 4-D TMA box per 64 columns, so a group's heads share every K/V tile.  A 128-key tile is fetched
+// page by page: lane i of the producer warp looks up its page one tile ahead and issues the box of
+// its gcd(page_size, 128) keys; boxes past the sequence's keys take an out-of-range page and fill with
+// zeros.  The slots between the last key and the end of its box may hold anything: the masked S
+// columns are replaced, and the MMA warp overwrites those V rows with zeros before the tile's PV.
+//
+//   warp 0      producer (whole warp): the run's items (published in a ring), Q tiles, K and V rings
+//   warp 1      TMEM allocator, MMA issuer:  S_A S_B | O_A += P_A V, S_A', O_B += P_B V, S_B' | ...
+//   warps 4-7   softmax of tile A, warps 8-11 of tile B: one row per thread, fp32 statistics, P (bf16)
+//               back into the S region of TMEM, O rescaled there when the maximum grows by over 2^8.
+//               A pair's last key tile may be past tile A's last key: A then ends earlier.
+//
+// TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
+#pragma once
+
+#include "attention.cuh"
+#include "paged.cuh"
+
+namespace beacon {
+
+template <int D>
+struct PagedTcCfg {
+  static constexpr uint32_t Q_BYTES = 128 * D * 2;
+  static constexpr uint32_t KV_BYTES = 128 * D * 2;
+  static constexpr int STAGES = D == 64 ? 4 : 2;  // K and V tiles in flight: 64 KB each
+  static constexpr size_t SMEM_BYTES = 1024 + 2 * (size_t)Q_BYTES + 2 * STAGES * (size_t)KV_BYTES + 1024;
+  static constexpr int THREADS = 384;
+};
+
+struct PagedTcParams {
+  PagedParams p;
+  float scale_log2;
+  int tpt;        // tokens per query tile
+  int box;        // keys per TMA box
+};
+
+enum : unsigned int {
+  kSitePtcItem = 0x621,
+  kSitePtcQ = 0x622,
+  kSitePtcKv = 0x623,
+  kSitePtcS = 0x624,
+  kSitePtcP = 0x625,
+  kSitePtcO = 0x626,
+  kSitePtcClean = 0x627,
+  kSitePtcDrain = 0x628,
+};
+
+constexpr int kPtcItems = 4;  // items published ahead
+struct PtcItem {
+  int valid;
+  int kvh, tok0;       // KV head; first token row of the item in q
+  int ntok;            // tokens from tok0 to the sequence's end
+  int lim0;            // keys that token tok0 sees (tok0 + i: lim0 + i), or kv when not causal
+  int kv;
+  int a, b;            // key tiles [a, b)
+  int end[2];          // the last key tile + 1 of tiles A, B within [a, b); <= a: none
+  int slot;            // workspace slot of a partial piece, -1: the whole item
+};
+
+// 2^a for a pair of arguments on the FMA pipe: a = n + f, f in [-0.5, 0.5], a quartic in f fitted to 2^f by
+// Lawson's iteration on the relative error (2.7e-6 in fp32), n added to the exponent.  The quartic, not
+// the cubic of the training forward, because lse is returned to 1e-5.  Arguments below -126 give less
+// than 2^-125.
+__device__ __forceinline__ void exp2_poly4(float& r0, float& r1, float a0, float a1) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
+  a0 = fmaxf(a0, -126.0f);
+  a1 = fmaxf(a1, -126.0f);
+  float t0, t1, n0, n1, f0, f1, p0, p1;
+  add2(t0, t1, a0, a1, kMagic, kMagic);
+  add2(n0, n1, t0, t1, -kMagic, -kMagic);
+  fma2(f0, f1, n0, n1, -1.0f, -1.0f, a0, a1);
+  fma2(p0, p1, 9.5701022e-3f, 9.5701022e-3f, f0, f1, 5.5917859e-2f, 5.5917859e-2f);
+  fma2(p0, p1, p0, p1, f0, f1, 2.4024744e-1f, 2.4024744e-1f);
+  fma2(p0, p1, p0, p1, f0, f1, 6.9312179e-1f, 6.9312179e-1f);
+  fma2(p0, p1, p0, p1, f0, f1, 9.9999928e-1f, 9.9999928e-1f);
+  r0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// P = 2^(x scale - m) of one 128-key row into the 64 TMEM columns at `taddr` (bf16 pairs); returns the
+// row's sum (fp32, before rounding).  Each 64-key half is handed to the MMA warp once stored.
+template <bool POLY>
+__device__ __forceinline__ float ptc_softmax(const float* x, float scale_log2, float neg_m, uint32_t taddr,
+                                             uint64_t* p_half) {
+  float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t pk[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      float a0, a1, p0, p1;
+      fma2(a0, a1, x[64 * c + 2 * e], x[64 * c + 2 * e + 1], scale_log2, scale_log2, neg_m, neg_m);
+      if (POLY && ((kPolyPairs >> (e & 7)) & 1u)) {
+        exp2_poly4(p0, p1, a0, a1);
+      } else {
+        p0 = ex2_approx(a0);
+        p1 = ex2_approx(a1);
+      }
+      const int q = 2 * (e & 1);
+      add2(ls[q], ls[q + 1], ls[q], ls[q + 1], p0, p1);
+      pk[e] = pack_bf16x2(p0, p1);
+    }
+    tmem_st32(taddr + 32 * c, pk);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane_id() == 0) mbar_arrive(&p_half[c]);
+  }
+  return (ls[0] + ls[1]) + (ls[2] + ls[3]);
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// Page of the box of keys that starts at `key`, or num_pages (outside the map: reads as zeros) when the
+// sequence has no such key or the table names no page of the cache.
+__device__ __forceinline__ int ptc_page(const PagedSeqs& g, int seq, int key, int kv) {
+  if (key >= kv) return g.num_pages;
+  const int page = __ldg(g.page_table + (long long)seq * g.table_stride + key / g.page_size);
+  if (page >= 0 && page < g.num_pages) return page;
+  record_fault(kFaultIndex, kSitePagedPage);
+  return g.num_pages;
+}
+
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    k_paged_attn_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const PagedTcParams tp) {
+  using Cfg = PagedTcCfg<D>;
+  constexpr int ST = Cfg::STAGES;
+  constexpr uint32_t LOG = ST == 2 ? 1 : 2;
+  const PagedParams& p = tp.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + 2 * Cfg::Q_BYTES;
+  uint8_t* sV = sK + ST * Cfg::KV_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::KV_BYTES);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = k_full + ST;
+  uint64_t* v_full = k_empty + ST;
+  uint64_t* v_empty = v_full + ST;
+  uint64_t* q_full = v_empty + ST;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;   // [2] per tile
+  uint64_t* p_full = s_full + 2;    // [2][2] per tile and 64-key half
+  uint64_t* o_full = p_full + 4;    // [2]
+  uint64_t* clean = o_full + 2;     // the MMA warp's lanes have zeroed a V tile's tail
+  uint64_t* drain = clean + 1;
+  uint64_t* item_full = drain + 1;               // [kPtcItems]
+  uint64_t* item_empty = item_full + kPtcItems;  // [kPtcItems] read by the MMA warp and 8 softmax warps
+  PtcItem* items = reinterpret_cast<PtcItem*>(item_empty + kPtcItems);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPtcItems);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t warp = warp_id(), lane = lane_id();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(clean, 32);
+    mbar_init(drain, 1);
+    for (int i = 0; i < kPtcItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 9);
+    }
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto read_item = [&](int ci, PtcItem& x) -> bool {
+    const int s = ci % kPtcItems;
+    if (!mbar_wait(&item_full[s], (uint32_t)(ci / kPtcItems) & 1u, abort_flag, kSitePtcItem)) return false;
+    x = items[s];
+    return x.valid != 0;
+  };
+
+  // 128 x 72 + 256 x 216 = 384 x 168, the allocation the CTA is launched with
+  if (warp < 4) {
+    warpgroup_reg_dealloc<72>();
+    if (warp == 0) {
+      // -------------------------------------------------------------- producer
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
+      }
+      PagedWalk walk;
+      walk.start(p, 128);
+      const int nbox = 128 / tp.box;
+      const uint32_t q_tile_bytes = (uint32_t)(tp.tpt * p.g) * 128u * (D / 64);
+      uint32_t tk = 0, kissued = 0, vissued = 0, kpar = 0, vpar = 0, qissued = 0, qpar = 0;
+      bool ok = true;
+      for (int ci = 0; ok; ++ci) {
+        PagedItem w{};
+        const bool more = walk.next(p, 128, w);
+        PtcItem x{};
+        x.valid = more ? 1 : 0;
+        if (more) {
+          const int t0 = w.row0 / p.g;
+          x.kvh = w.kvh;
+          x.tok0 = w.q0 + t0;
+          x.ntok = w.q_len - t0;
+          x.lim0 = p.causal ? w.kv - w.q_len + t0 + 1 : w.kv;
+          x.kv = w.kv;
+          x.a = w.a;
+          x.b = w.b;
+          x.slot = (w.a == 0 && w.b == w.n) ? -1 : paged_slot(w);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int last = min((t + 1) * tp.tpt, x.ntok) - 1;
+            const int keys = p.causal ? max(0, x.lim0 + last) : x.kv;
+            x.end[t] = t * tp.tpt < x.ntok ? min(w.b, max(1, (keys + 127) / 128)) : 0;
+          }
+        }
+        const int is = ci % kPtcItems;
+        ok = warp_wait(&item_empty[is], ((uint32_t)(ci / kPtcItems) & 1u) ^ 1u, abort_flag, kSitePtcItem);
+        if (!ok) break;
+        if (lane == 0) {
+          items[is] = x;
+          mbar_arrive(&item_full[is]);
+          if (more && w.a == 0 && w.b < w.n) p.heads[blockIdx.x] = paged_head(p, w, walk.chunk);
+        }
+        if (!more) break;
+        int page = (int)lane < nbox ? ptc_page(p.pg, w.seq, x.a * 128 + (int)lane * tp.box, w.kv) : 0;
+        ok = warp_wait(q_empty, ((uint32_t)ci & 1u) ^ 1u, abort_flag, kSitePtcQ);
+        if (!ok) break;
+        if (lane == 0) {
+          const int nt = x.end[1] > x.a ? 2 : 1, first = x.end[0] > x.a ? 0 : 1;
+          mbar_arrive_expect_tx(q_full, (uint32_t)(nt - first) * q_tile_bytes);
+          for (int t = first; t < nt; ++t)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(sQ + t * Cfg::Q_BYTES + c * 16384, &tmQ, q_full, c * 64, 0, x.tok0 + t * tp.tpt, x.kvh);
+        }
+        qissued = 1;
+        qpar = (uint32_t)ci & 1u;
+        for (int j = x.a; j < x.b; ++j, ++tk) {
+          const uint32_t st = tk & (ST - 1), ph = (tk >> LOG) & 1u;
+          const int key = j * 128 + (int)lane * tp.box, cur = page;
+          if (j + 1 < x.b && (int)lane < nbox) page = ptc_page(p.pg, w.seq, key + 128, w.kv);
+          const int row = key % p.pg.page_size;
+          ok = warp_wait(&k_empty[st], ph ^ 1u, abort_flag, kSitePtcKv);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&k_full[st], Cfg::KV_BYTES);
+          __syncwarp();
+          if ((int)lane < nbox) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(sK + st * Cfg::KV_BYTES + c * 16384 + lane * tp.box * 128, &tmK, &k_full[st], c * 64, row,
+                          x.kvh, cur);
+          }
+          kissued |= 1u << st;
+          kpar = (kpar & ~(1u << st)) | (ph << st);
+          ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, kSitePtcKv);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&v_full[st], Cfg::KV_BYTES);
+          __syncwarp();
+          if ((int)lane < nbox) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(sV + st * Cfg::KV_BYTES + c * 16384 + lane * tp.box * 128, &tmV, &v_full[st], c * 64, row,
+                          x.kvh, cur);
+          }
+          vissued |= 1u << st;
+          vpar = (vpar & ~(1u << st)) | (ph << st);
+        }
+      }
+      if (!ok && lane == 0) {  // a wait gave up: the copies in flight land before the CTA may end
+        volatile int no_abort = 0;
+        if (qissued) mbar_wait(q_full, qpar, &no_abort, kSitePtcDrain);
+        for (int s = 0; s < ST; ++s) {
+          if (kissued & (1u << s)) mbar_wait(&k_full[s], (kpar >> s) & 1u, &no_abort, kSitePtcDrain);
+          if (vissued & (1u << s)) mbar_wait(&v_full[s], (vpar >> s) & 1u, &no_abort, kSitePtcDrain);
+        }
+      }
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- MMA issuer
+      const bool leader = elect_one();
+      constexpr uint32_t idesc_s = make_idesc_f16(128, 128, false, false);
+      constexpr uint32_t idesc_o = make_idesc_f16(128, D, false, true);
+      const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = make_sdesc_sw128(smem_u32(sK), 16, 1024);
+      const uint64_t v_desc = make_sdesc_sw128(smem_u32(sV), 128 * 128, 1024);
+      auto issue_s = [&](int t, uint32_t k) {
+        const uint64_t qd = sdesc_adv(q_desc, t * Cfg::Q_BYTES), kd = sdesc_adv(k_desc, (k & (ST - 1)) * Cfg::KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+          if (leader) umma_f16_ss(tmem + 128 * t, sdesc_adv(qd, off), sdesc_adv(kd, off), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        if (leader) umma_commit(&s_full[t]);
+      };
+      uint32_t tk = 0, ns[2] = {0u, 0u}, nclean = 0;
+      bool ok = true;
+      PtcItem x;
+      // per-lane waits inside an item, as in k_attn_fwd_tc: no warp collective until its end
+      for (int ci = 0;; ++ci) {
+        const bool got = ok && read_item(ci, x);
+        if (!__all_sync(0xffffffffu, got)) break;
+        const int n = x.b - x.a;
+        const int tail = x.kv & 127;                                        // keys in the sequence's last tile
+        const int dirty = tail % tp.box != 0 ? x.kv >> 7 : -1;              // the tile whose V rows need zeros
+        const int dirty_end = tail + (tp.box - tail % tp.box);
+        bool iok = lane_wait(q_full, (uint32_t)ci & 1u, abort_flag, kSitePtcQ) &&
+                   lane_wait(&k_full[tk & (ST - 1)], (tk >> LOG) & 1u, abort_flag, kSitePtcKv);
+        if (iok) {
+          tc_fence_after();
+          for (int t = 0; t < 2; ++t)
+            if (x.end[t] > x.a) issue_s(t, tk);
+          if (leader) umma_commit(&k_empty[tk & (ST - 1)]);
+          if (n == 1 && leader) umma_commit(q_empty);
+        }
+        for (int i = 0; i < n && iok; ++i) {
+          const int j = x.a + i;
+          const uint32_t tv = tk + (uint32_t)i, tn = tv + 1u;
+          bool k_next = false;
+          if (!lane_wait(&v_full[tv & (ST - 1)], (tv >> LOG) & 1u, abort_flag, kSitePtcKv)) { iok = false; break; }
+          if (j == dirty) {
+            uint8_t* vt = sV + (tv & (ST - 1)) * Cfg::KV_BYTES;
+            const int chunks = (dirty_end - tail) * 8;
+            for (int e = (int)lane; e < chunks * (D / 64); e += 32) {
+              const int c = e / chunks, o = e - c * chunks;
+              *reinterpret_cast<uint4*>(vt + c * 16384 + tail * 128 + o * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(clean);
+            if (!lane_wait(clean, nclean & 1u, abort_flag, kSitePtcClean)) { iok = false; break; }
+            ++nclean;
+          }
+          const uint64_t vd = sdesc_adv(v_desc, (tv & (ST - 1)) * Cfg::KV_BYTES);
+          for (int t = 0; t < 2 && iok; ++t) {
+            if (j >= x.end[t]) continue;
+            for (int hf = 0; hf < 2 && iok; ++hf) {
+              if (!lane_wait(&p_full[2 * t + hf], (ns[t] + (uint32_t)i) & 1u, abort_flag, kSitePtcP)) {
+                iok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) {
+                const int kk = 4 * hf + k4;
+                if (leader)
+                  umma_f16_ts(tmem + 256 + t * D, tmem + 128 * t + kk * 8, sdesc_adv(vd, kk * 2048), idesc_o,
+                              (i > 0 || kk > 0) ? 1u : 0u);
+              }
+            }
+            if (!iok) break;
+            if (j == x.end[t] - 1 && leader) umma_commit(&o_full[t]);
+            if (j + 1 < x.end[t]) {
+              if (!k_next) {
+                if (!lane_wait(&k_full[tn & (ST - 1)], (tn >> LOG) & 1u, abort_flag, kSitePtcKv)) { iok = false; break; }
+                tc_fence_after();
+                k_next = true;
+              }
+              issue_s(t, tn);
+            }
+          }
+          if (!iok) break;
+          if (leader) umma_commit(&v_empty[tv & (ST - 1)]);
+          if (k_next && leader) umma_commit(&k_empty[tn & (ST - 1)]);
+          if (i + 2 == n && leader) umma_commit(q_empty);
+        }
+        ok = iok;
+        tk += (uint32_t)n;
+        for (int t = 0; t < 2; ++t) ns[t] += (uint32_t)max(0, x.end[t] - x.a);
+        __syncwarp();
+        if (ok && leader) mbar_arrive(&item_empty[ci % kPtcItems]);
+      }
+      if (leader) umma_commit(drain);
+      volatile int no_abort = 0;
+      warp_wait(drain, 0, &no_abort, kSitePtcDrain);
+    }
+  } else {
+    warpgroup_reg_alloc<216>();
+    // ---------------------------------------------------------------- softmax
+    const int t = warp < 8 ? 0 : 1;
+    const int r = (int)((warp & 3u) * 32 + lane);
+    const uint32_t lane_base = ((warp & 3u) * 32u) << 16;
+    const uint32_t s_col = 128 * t, o_col = 256 + t * D;
+    const int rt = r / p.g;  // token of the tile
+    const bool in_tile = rt < tp.tpt;
+    const int head = r - rt * p.g;
+    uint32_t ns = 0, no = 0;
+    bool ok = true;
+    for (int ci = 0; ok; ++ci) {
+      PtcItem x;
+      const bool more = __all_sync(0xffffffffu, read_item(ci, x));
+      if (lane == 0) mbar_arrive(&item_empty[ci % kPtcItems]);
+      if (!more) break;
+      const int end = x.end[t], tok = t * tp.tpt + rt;
+      const bool row_ok = in_tile && tok < x.ntok;
+      // rows that are stored nowhere count as seeing every key, so that they do not force the masked path
+      const int lim = !row_ok ? INT32_MAX : p.causal ? max(0, x.lim0 + tok) : x.kv;
+      float m_used = -INFINITY, l = 0.0f;
+      for (int j = x.a; j < end; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (ns + (uint32_t)(j - x.a)) & 1u, abort_flag, kSitePtcS))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t xu[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld32(tmem + lane_base + s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&xu[32 * c]));
+        tmem_wait_ld();
+        float* xs = reinterpret_cast<float*>(xu);
+        const int limit = lim - j * 128;
+        const bool unmasked = __all_sync(0xffffffffu, limit >= 128);
+        if (!unmasked) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) xs[c] = (c < limit) ? xs[c] : -INFINITY;
+        }
+        float m8[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m8[u] = fmaxf(xs[u], xs[8 + u]);
+#pragma unroll
+        for (int c = 16; c < 128; c += 16)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) m8[u] = fmax3(m8[u], xs[c + u], xs[c + 8 + u]);
+        const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
+                         tp.scale_log2;
+        const float m_new = fmaxf(m_used, mx);
+        if (j == x.a) {
+          m_used = m_new;
+        } else {
+          // a row without a key so far has O = 0 and m = -inf: 2^(-inf) = 0 rescales it
+          const bool need = m_new > m_used + 8.0f;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? ex2_approx(m_used - m_new) : 1.0f;
+            if (need) {
+              l *= alpha;
+              m_used = m_new;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t u[32];
+              tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * alpha);
+              tmem_st32(tmem + lane_base + o_col + c * 32, u);
+            }
+          }
+        }
+        const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
+        if (unmasked)
+          l += ptc_softmax<true>(xs, tp.scale_log2, neg_m, tmem + lane_base + s_col, &p_full[2 * t]);
+        else
+          l += ptc_softmax<false>(xs, tp.scale_log2, neg_m, tmem + lane_base + s_col, &p_full[2 * t]);
+      }
+      if (!ok) break;
+      ns += (uint32_t)max(0, end - x.a);
+      const int row = t * tp.tpt * p.g + r;  // row of the item
+      if (end <= x.a) {  // this piece holds no key of the tile's rows
+        if (x.slot >= 0 && row_ok) p.part_ml[(long long)x.slot * p.rpi + row] = make_float2(-INFINITY, 0.0f);
+        continue;
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1u, abort_flag, kSitePtcO))) {
+        ok = false;
+        break;
+      }
+      ++no;
+      tc_fence_after();
+      if (x.slot < 0) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const bool none = m_used == -INFINITY;
+        const long long at = (long long)(x.tok0 + tok) * p.Hq + (long long)x.kvh * p.g + head;
+        __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.out) + at * D;
+        const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t u[32];
+          tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+          tmem_wait_ld();
+          if (!row_ok) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t wv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              wv[i] = none ? 0u
+                           : pack_bf16x2(__uint_as_float(u[e + 2 * i]) * inv, __uint_as_float(u[e + 2 * i + 1]) * inv);
+            if (out32) {
+              stg256(orow + c * 32 + e, wv[0], wv[1], wv[2], wv[3], wv[4], wv[5], wv[6], wv[7]);
+            } else {
+              *reinterpret_cast<uint4*>(orow + c * 32 + e) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+              *reinterpret_cast<uint4*>(orow + c * 32 + e + 8) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
+            }
+          }
+        }
+        if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
+      } else {
+        float* po = p.part_o + ((long long)x.slot * p.rpi + row) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t u[32];
+          tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+          tmem_wait_ld();
+          if (!row_ok) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            stg256(po + c * 32 + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+        }
+        if (row_ok) p.part_ml[(long long)x.slot * p.rpi + row] = make_float2(m_used, l);
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace beacon

@@ -1,0 +1,603 @@
+// rope.cuh -- RMS norm of each query and key head and the position rotation in one pass,
+// between the QKV projection (rows of (Hq + 2 Hkv) heads per token) and attention:
+// head-major tensors for training, token-major queries and a paged key/value cache for
+// serving, and the backward of the training form.
+//
+// One head x[D] of a token at position t, gain g[D] (optional), rot rotated dims (even):
+//   r = sqrt(mean x^2 + eps), z = g x / r,
+//   y_a = z_a c_i - z_b s_i, y_b = z_b c_i + z_a s_i, i < rot / 2,  y_d = z_d for d >= rot,
+// with (a, b) = (i, i + rot/2), or (2i, 2i+1) interleaved, and (c_i, s_i) = the table's row t
+// (rot/2 cosines, then rot/2 sines).  Without a gain z = x (rotation only).  Backward, dz the
+// rotation of dy by the opposite angle:
+//   dg += sum dz x / r,  e = g dz,  dx = e / r - x sum(e x) / (D r^3)   (dx = dz without a gain).
+// Bound: HBM (each head is read once and written once; ~10 FLOP per element).
+#pragma once
+
+#include "elementwise.cuh"
+#include "sm100.cuh"
+
+namespace beacon {
+
+// A batch of sequences whose keys and values live in pages: sequence s owns the new tokens
+// [cu_q[s], cu_q[s+1]) of the token-major tensors and kv_lens[s] tokens of the cache, the
+// new ones included and last; its j-th token sits in slot j % page_size of page
+// page_table[s][j / page_size].
+struct PagedSeqs {
+  const int* cu_q;        // [seqs + 1]
+  const int* kv_lens;     // [seqs]
+  const int* page_table;  // [seqs, table_stride]
+  long long table_stride;
+  int seqs, max_pages, num_pages, page_size;
+  long long page_stride, head_stride, token_stride;  // of both caches, in elements
+};
+
+struct RopeParams {
+  int Hq, Hkv, D, rot, interleaved;
+  float eps;
+  long long tokens;
+  int seq;                 // head-major forms: tokens per batch entry
+  const float* table;      // [table_positions, rot]
+  long long table_positions;
+  const int* positions;    // [tokens] or null (token % seq, or the token's place in its sequence)
+  long long ld;            // elements between token rows of qkv (and of dqkv: ld_out)
+  long long ld_out;
+  PagedSeqs pg;            // paged form
+};
+
+enum : unsigned int {
+  kSiteRopePosition = 0x601,  // a position outside the table, or before the sequence's start
+  kSiteRopePage = 0x602,      // a page index outside the cache, or a token past the page table
+};
+
+// Number of i in [1, n] with cu[i] <= t (the sequence that owns token t; n: none does).
+// Whole warp, 32-way: two dependent loads up to 1024 sequences.
+__device__ __forceinline__ int warp_owner(const int* __restrict__ cu, int n, long long t) {
+  const int lane = (int)lane_id();
+  int lo = 0;
+  while (n > 0) {
+    const int step = (n + 31) >> 5;
+    const bool on = (long long)lane * step < n;
+    const int at = min((lane + 1) * step, n);
+    const bool le = on && (long long)__ldg(cu + lo + at) <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, le));
+    const int active = __popc(__ballot_sync(0xffffffffu, on));
+    const int skip = min(c * step, n);
+    n = c < active ? min((c + 1) * step, n) - skip - 1 : 0;
+    lo += skip;
+  }
+  return lo;
+}
+
+// Where a token goes: its rotation row, and the element offset of its slot for KV head 0.
+struct TokenPlace {
+  bool on;          // the token belongs to a sequence (paged form)
+  long long pos;    // table row, -1: none (the head rows are written as zeros)
+  long long slot;   // paged form: cache offset of (page, head 0, token), -1: nowhere
+};
+template <bool PAGED>
+__device__ __forceinline__ TokenPlace token_place(const RopeParams& p, long long t) {
+  TokenPlace w{true, 0, -1};
+  if constexpr (PAGED) {
+    const PagedSeqs& g = p.pg;
+    const int s = warp_owner(g.cu_q, g.seqs, t);
+    if (s >= g.seqs || t < (long long)__ldg(g.cu_q)) {
+      w.on = false;
+      return w;
+    }
+    const long long at = (long long)__ldg(g.kv_lens + s) - ((long long)__ldg(g.cu_q + s + 1) - t);
+    w.pos = at;
+    if (at >= 0) {
+      const long long pi = at / g.page_size;
+      int page = -1;
+      if (pi < g.max_pages) page = __ldg(g.page_table + (long long)s * g.table_stride + pi);
+      if (page >= 0 && page < g.num_pages)
+        w.slot = (long long)page * g.page_stride + (at - pi * g.page_size) * g.token_stride;
+      else if (lane_id() == 0)
+        record_fault(kFaultIndex, kSiteRopePage);
+    }
+  } else {
+    w.pos = t % p.seq;
+  }
+  if (p.positions != nullptr && w.pos >= 0) w.pos = __ldg(p.positions + t);
+  if (w.pos < 0 || w.pos >= p.table_positions) {
+    if (lane_id() == 0) record_fault(kFaultIndex, kSiteRopePosition);
+    w.pos = -1;
+  }
+  return w;
+}
+
+// Destination of head h (0 .. Hq + 2 Hkv) of token t; null: not written.
+template <typename T, bool PAGED>
+__device__ __forceinline__ T* head_out(const RopeParams& p, const TokenPlace& w, long long t, int h, T* q, T* k, T* v) {
+  if constexpr (PAGED) {
+    if (h < p.Hq) return q + (t * p.Hq + h) * p.D;
+    if (w.slot < 0) return nullptr;
+    h -= p.Hq;
+    T* base = h < p.Hkv ? k : v;
+    return base + w.slot + (long long)(h < p.Hkv ? h : h - p.Hkv) * p.pg.head_stride;
+  } else {
+    const long long b = t / p.seq, s = t - b * p.seq;
+    if (h < p.Hq) return q + ((b * p.Hq + h) * p.seq + s) * p.D;
+    h -= p.Hq;
+    T* base = h < p.Hkv ? k : v;
+    if (base == nullptr) return nullptr;
+    return base + ((b * p.Hkv + (h < p.Hkv ? h : h - p.Hkv)) * p.seq + s) * p.D;
+  }
+}
+
+// Rotation partner of element d (d < rot) and the pair's index; first: d is the pair's first member.
+__device__ __forceinline__ void rope_pair(int d, int rot, int interleaved, int& i, int& partner, bool& first) {
+  const int half = rot >> 1;
+  if (interleaved) {
+    i = d >> 1;
+    partner = d ^ 1;
+    first = (d & 1) == 0;
+  } else {
+    first = d < half;
+    i = first ? d : d - half;
+    partner = first ? d + half : d - half;
+  }
+}
+
+// Any head_dim up to kRopeMaxDim, any alignment: one warp per (token, head), element by element,
+// the row read a second time from L1 for the rotation.
+constexpr int kRopeMaxDim = 256;
+template <typename T, bool PAGED>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_any(T* __restrict__ q, T* __restrict__ k, T* __restrict__ v,
+                                                          const T* __restrict__ qkv, const T* __restrict__ q_gain,
+                                                          const T* __restrict__ k_gain, const RopeParams p) {
+  const int lane = (int)lane_id();
+  const int heads = p.Hq + 2 * p.Hkv;
+  const long long n = p.tokens * heads, warps = (long long)gridDim.x * (blockDim.x >> 5);
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
+    const long long t = u / heads;
+    const int h = (int)(u - t * heads);
+    const TokenPlace w = token_place<PAGED>(p, t);
+    if (!w.on) continue;
+    T* o = head_out<T, PAGED>(p, w, t, h, q, k, v);
+    if (o == nullptr) continue;
+    const T* x = qkv + t * p.ld + (long long)h * p.D;
+    if (h >= p.Hq + p.Hkv) {
+      for (int d = lane; d < p.D; d += 32) o[d] = x[d];
+      continue;
+    }
+    const T* g = h < p.Hq ? q_gain : k_gain;
+    float inv = 1.0f;
+    if (g != nullptr) {
+      float ss = 0.0f;
+      for (int d = lane; d < p.D; d += 32) ss = fmaf(ldf(x + d), ldf(x + d), ss);
+      inv = 1.0f / sqrtf(warp_sum(ss) / (float)p.D + p.eps);
+    }
+    const float* tab = p.table + w.pos * p.rot;
+    for (int d = lane; d < p.D; d += 32) {
+      float y = w.pos < 0 ? 0.0f : ldf(x + d) * inv * (g != nullptr ? ldf(g + d) : 1.0f);
+      if (w.pos >= 0 && d < p.rot) {
+        int i, e;
+        bool first;
+        rope_pair(d, p.rot, p.interleaved, i, e, first);
+        const float z = ldf(x + e) * inv * (g != nullptr ? ldf(g + e) : 1.0f);
+        const float c = __ldg(tab + i), s = __ldg(tab + (p.rot >> 1) + i);
+        y = first ? y * c - z * s : y * c + z * s;
+      }
+      stf(o + d, y);
+    }
+  }
+}
+
+// Backward, same mapping; part: [gridDim.x, 2, D] partial sums of dq_gain and dk_gain (fp32), each
+// CTA's warps added in warp order, or null.
+template <typename T>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dqkv, float* __restrict__ part,
+                                                              const T* __restrict__ dq, const T* __restrict__ dk,
+                                                              const T* __restrict__ dv, const T* __restrict__ qkv,
+                                                              const T* __restrict__ q_gain,
+                                                              const T* __restrict__ k_gain, const RopeParams p) {
+  __shared__ float red[8][kRopeMaxDim];
+  const int lane = (int)lane_id(), warp = (int)warp_id();
+  const int heads = p.Hq + 2 * p.Hkv;
+  const long long n = p.tokens * heads, warps = (long long)gridDim.x * (blockDim.x >> 5);
+  float acc[2][kRopeMaxDim / 32] = {};
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
+    const long long t = u / heads;
+    const int h = (int)(u - t * heads);
+    const TokenPlace w = token_place<false>(p, t);
+    const T* dy = head_out<const T, false>(p, w, t, h, dq, dk, dv);
+    if (dy == nullptr) continue;
+    T* o = dqkv + t * p.ld_out + (long long)h * p.D;
+    if (h >= p.Hq + p.Hkv) {
+      for (int d = lane; d < p.D; d += 32) o[d] = dy[d];
+      continue;
+    }
+    const T* x = qkv + t * p.ld + (long long)h * p.D;
+    const int kind = h < p.Hq ? 0 : 1;
+    const T* g = kind == 0 ? q_gain : k_gain;
+    const float* tab = p.table + w.pos * p.rot;
+    float dz[kRopeMaxDim / 32], ss = 0.0f, ex = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kRopeMaxDim / 32; ++j) {
+      const int d = lane + 32 * j;
+      dz[j] = 0.0f;
+      if (d >= p.D || w.pos < 0) continue;
+      dz[j] = ldf(dy + d);
+      if (d < p.rot) {
+        int i, e;
+        bool first;
+        rope_pair(d, p.rot, p.interleaved, i, e, first);
+        const float c = __ldg(tab + i), s = __ldg(tab + (p.rot >> 1) + i);
+        dz[j] = first ? dz[j] * c + ldf(dy + e) * s : dz[j] * c - ldf(dy + e) * s;
+      }
+      if (g != nullptr) {
+        const float xv = ldf(x + d);
+        ss = fmaf(xv, xv, ss);
+        ex = fmaf(dz[j] * ldf(g + d), xv, ex);
+      }
+    }
+    float inv = 1.0f, back = 0.0f;
+    if (g != nullptr && w.pos >= 0) {
+      ss = warp_sum(ss);
+      ex = warp_sum(ex);
+      inv = 1.0f / sqrtf(ss / (float)p.D + p.eps);
+      back = ex * inv * inv / (float)p.D;
+    }
+#pragma unroll
+    for (int j = 0; j < kRopeMaxDim / 32; ++j) {
+      const int d = lane + 32 * j;
+      if (d >= p.D) continue;
+      if (g == nullptr) {
+        stf(o + d, dz[j]);
+      } else {
+        const float xv = ldf(x + d);
+        if (w.pos >= 0) {
+          const float add = dz[j] * xv * inv;
+          if (kind == 0) acc[0][j] += add;
+          else acc[1][j] += add;
+        }
+        stf(o + d, w.pos < 0 ? 0.0f : inv * (dz[j] * ldf(g + d) - xv * back));
+      }
+    }
+  }
+  if (part == nullptr) return;
+  for (int kind = 0; kind < 2; ++kind) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kRopeMaxDim / 32; ++j) red[warp][lane + 32 * j] = kind == 0 ? acc[0][j] : acc[1][j];
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.D; d += blockDim.x) {
+      float s = 0.0f;
+      for (int w = 0; w < 8; ++w) s += red[w][d];
+      part[((long long)blockIdx.x * 2 + kind) * p.D + d] = s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Vectorised forms: head_dim 16 .. 256 (a power of two), rot % 16 == 0, 16-byte aligned rows.
+//
+// A head takes D/16 lanes, each holding two 8-element chunks rot/2 apart, so that both members of a
+// rotated pair sit in one lane (halves or interleaved) and the only exchange is the sum over the
+// head's lanes; the lanes behind rot/16 hold the pass-through elements the same way.  A warp keeps
+// one batch of U * 32/(D/16) heads of one kind (query, key or value) for every token it visits: its
+// gains stay in registers and a token's cosines and sines are loaded once per batch.
+// ---------------------------------------------------------------------------
+struct RopeBatches {
+  int nq, nk;  // batches of query heads, of key heads (value heads: as many as key heads)
+  __host__ __device__ int total() const { return nq + 2 * nk; }
+};
+
+// Elements [e0, e0+8) and [e1, e1+8) of a head are lane l's; turns: they are rotated.
+template <int D>
+struct RopeLane {
+  int sub, l, e0, e1;  // head of the warp's 32/(D/16), lane within it
+  bool turns;
+  __device__ __forceinline__ explicit RopeLane(int rot) {
+    constexpr int LPH = D / 16;
+    const int lane = (int)lane_id();
+    l = lane % LPH;
+    sub = lane / LPH;
+    turns = l < rot / 16;
+    e0 = turns ? 8 * l : rot + 8 * (l - rot / 16);
+    e1 = e0 + (turns ? rot / 2 : (D - rot) / 2);
+  }
+  // Sum over the head's lanes.
+  __device__ __forceinline__ float sum(float v) const {
+#pragma unroll
+    for (int o = D / 32; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  // Cosines and sines of the lane's eight pairs (1, 0 where nothing turns).  Halves: pair i joins
+  // elements i of the two chunks; interleaved: pairs 0-3 lie in the first chunk, 4-7 in the second.
+  __device__ __forceinline__ void turn(const RopeParams& p, long long pos, float (&c)[8], float (&s)[8]) const {
+    if (!turns || pos < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = 1.0f;
+        s[i] = 0.0f;
+      }
+      return;
+    }
+    const float* tab = p.table + pos * p.rot;
+    const int i0 = p.interleaved ? e0 >> 1 : e0, i1 = p.interleaved ? e1 >> 1 : e0 + 4;
+    const int half = p.rot >> 1;
+    const float4 c0 = __ldg(reinterpret_cast<const float4*>(tab + i0));
+    const float4 c1 = __ldg(reinterpret_cast<const float4*>(tab + i1));
+    const float4 s0 = __ldg(reinterpret_cast<const float4*>(tab + half + i0));
+    const float4 s1 = __ldg(reinterpret_cast<const float4*>(tab + half + i1));
+    c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
+    s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
+  }
+};
+
+// (a, b) = the lane's 16 elements turned by the pairs' angles; `back`: by the opposite angles.
+__device__ __forceinline__ void rope_turn(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8],
+                                          bool interleaved, bool back) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float sn = back ? -s[i] : s[i];
+    if (interleaved) {
+      float& x = i < 4 ? a[2 * i] : b[2 * i - 8];
+      float& y = i < 4 ? a[2 * i + 1] : b[2 * i - 7];
+      const float u = x * c[i] - y * sn, w = y * c[i] + x * sn;
+      x = u;
+      y = w;
+    } else {
+      const float u = a[i] * c[i] - b[i] * sn, w = b[i] * c[i] + a[i] * sn;
+      a[i] = u;
+      b[i] = w;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void ldraw_cs(const T* p, Raw8<T>& r) {  // read once: evict first
+#pragma unroll
+  for (int k = 0; k < (int)(sizeof(T) / 2); ++k) r.u[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+}
+template <typename T>
+__device__ __forceinline__ void straw(T* p, const Raw8<T>& r) {
+#pragma unroll
+  for (int k = 0; k < (int)(sizeof(T) / 2); ++k) reinterpret_cast<uint4*>(p)[k] = r.u[k];
+}
+
+template <typename T, int D, int U, bool PAGED>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_vec(T* __restrict__ q, T* __restrict__ k, T* __restrict__ v,
+                                                          const T* __restrict__ qkv, const T* __restrict__ q_gain,
+                                                          const T* __restrict__ k_gain, const RopeParams p,
+                                                          const RopeBatches nb) {
+  constexpr int HPW = 32 / (D / 16);
+  const RopeLane<D> ln(p.rot);
+  const int n = nb.total();
+  const unsigned gw = blockIdx.x * 8u + warp_id(), warps = gridDim.x * 8u;
+  const int b = (int)(gw % (unsigned)n), step = (int)(warps / (unsigned)n);
+  if (gw >= (unsigned)n * (unsigned)step) return;  // warps beyond a whole number of rounds
+  const int kind = b < nb.nq ? 0 : b < nb.nq + nb.nk ? 1 : 2;  // query, key, value heads
+  const int h0 = (kind == 0 ? b : kind == 1 ? b - nb.nq : b - nb.nq - nb.nk) * (U * HPW) + ln.sub;
+  const int count = kind == 0 ? p.Hq : p.Hkv;
+  const int col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
+  const T* gain = kind == 0 ? q_gain : kind == 1 ? k_gain : nullptr;
+  Raw8<T> g0, g1;
+  if (gain != nullptr) {
+    ldraw(gain + ln.e0, g0);
+    ldraw(gain + ln.e1, g1);
+  }
+  for (long long t = gw / (unsigned)n; t < p.tokens; t += step) {
+    const T* row = qkv + t * p.ld + (long long)col * D;
+    Raw8<T> x0[U], x1[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW;
+      if (h < count) {
+        ldraw_cs(row + (long long)h * D + ln.e0, x0[u]);
+        ldraw_cs(row + (long long)h * D + ln.e1, x1[u]);
+      }
+    }
+    const TokenPlace w = token_place<PAGED>(p, t);
+    if (!w.on) continue;
+    if (kind == 2) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * HPW;
+        T* o = h < count ? head_out<T, PAGED>(p, w, t, col + h, q, k, v) : nullptr;
+        if (o == nullptr) continue;
+        straw(o + ln.e0, x0[u]);
+        straw(o + ln.e1, x1[u]);
+      }
+      continue;
+    }
+    float c[8], s[8];
+    ln.turn(p, w.pos, c, s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW;
+      float a[8], z[8];
+      unraw(x0[u], a);
+      unraw(x1[u], z);
+      if (gain != nullptr) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(z[i], z[i], ss));
+        const float inv = 1.0f / sqrtf(ln.sum(ss) * (1.0f / D) + p.eps);
+        float ga[8], gz[8];
+        unraw(g0, ga);
+        unraw(g1, gz);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[i] = a[i] * inv * ga[i];
+          z[i] = z[i] * inv * gz[i];
+        }
+      }
+      if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, false);
+      if (w.pos < 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
+      }
+      T* o = h < count ? head_out<T, PAGED>(p, w, t, col + h, q, k, v) : nullptr;
+      if (o == nullptr) continue;
+      store8(o + ln.e0, a);
+      store8(o + ln.e1, z);
+    }
+  }
+}
+
+// Backward; part as in k_qk_norm_rope_bwd_any.  A warp keeps the partial sums of its kind's gain
+// gradient for its 16 columns in registers over all its tokens.
+template <typename T, int D, int U>
+__global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_vec(T* __restrict__ dqkv, float* __restrict__ part,
+                                                              const T* __restrict__ dq, const T* __restrict__ dk,
+                                                              const T* __restrict__ dv, const T* __restrict__ qkv,
+                                                              const T* __restrict__ q_gain,
+                                                              const T* __restrict__ k_gain, const RopeParams p,
+                                                              const RopeBatches nb) {
+  constexpr int HPW = 32 / (D / 16);
+  __shared__ float red[8][D];
+  __shared__ int kinds[8];
+  const RopeLane<D> ln(p.rot);
+  const int n = nb.total();
+  const unsigned gw = blockIdx.x * 8u + warp_id(), warps = gridDim.x * 8u;
+  const int b = (int)(gw % (unsigned)n), step = (int)(warps / (unsigned)n);
+  const bool on = gw < (unsigned)n * (unsigned)step;
+  const int kind = b < nb.nq ? 0 : b < nb.nq + nb.nk ? 1 : 2;
+  const int h0 = (kind == 0 ? b : kind == 1 ? b - nb.nq : b - nb.nq - nb.nk) * (U * HPW) + ln.sub;
+  const int count = kind == 0 ? p.Hq : p.Hkv;
+  const int col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
+  const T* gain = kind == 0 ? q_gain : kind == 1 ? k_gain : nullptr;
+  Raw8<T> g0, g1;
+  if (gain != nullptr) {
+    ldraw(gain + ln.e0, g0);
+    ldraw(gain + ln.e1, g1);
+  }
+  float acc0[8] = {}, acc1[8] = {};
+  for (long long t = on ? gw / (unsigned)n : p.tokens; t < p.tokens; t += step) {
+    const TokenPlace w = token_place<false>(p, t);
+    Raw8<T> y0[U], y1[U], x0[U], x1[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW;
+      if (h >= count) continue;
+      const T* dy = head_out<const T, false>(p, w, t, col + h, dq, dk, dv);
+      if (dy == nullptr) continue;
+      ldraw_cs(dy + ln.e0, y0[u]);
+      ldraw_cs(dy + ln.e1, y1[u]);
+      if (gain != nullptr) {
+        const T* x = qkv + t * p.ld + (long long)(col + h) * D;
+        ldraw_cs(x + ln.e0, x0[u]);
+        ldraw_cs(x + ln.e1, x1[u]);
+      }
+    }
+    T* row = dqkv + t * p.ld_out + (long long)col * D;
+    if (kind == 2) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * HPW;
+        if (h >= count || dv == nullptr) continue;
+        straw(row + (long long)h * D + ln.e0, y0[u]);
+        straw(row + (long long)h * D + ln.e1, y1[u]);
+      }
+      continue;
+    }
+    float c[8], s[8];
+    ln.turn(p, w.pos, c, s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW;
+      float a[8], z[8];
+      unraw(y0[u], a);
+      unraw(y1[u], z);
+      if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, true);
+      if (gain != nullptr) {
+        float xa[8], xz[8], ga[8], gz[8], ss = 0.0f, ex = 0.0f;
+        unraw(x0[u], xa);
+        unraw(x1[u], xz);
+        unraw(g0, ga);
+        unraw(g1, gz);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = fmaf(xa[i], xa[i], fmaf(xz[i], xz[i], ss));
+          ex = fmaf(a[i] * ga[i], xa[i], fmaf(z[i] * gz[i], xz[i], ex));
+        }
+        const float inv = 1.0f / sqrtf(ln.sum(ss) * (1.0f / D) + p.eps);
+        const float back = ln.sum(ex) * inv * inv * (1.0f / D);
+        const float wgt = (h < count && w.pos >= 0) ? inv : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (wgt != 0.0f) {
+            acc0[i] = fmaf(a[i] * wgt, xa[i], acc0[i]);
+            acc1[i] = fmaf(z[i] * wgt, xz[i], acc1[i]);
+          }
+          a[i] = inv * (a[i] * ga[i] - xa[i] * back);
+          z[i] = inv * (z[i] * gz[i] - xz[i] * back);
+        }
+      }
+      if (w.pos < 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
+      }
+      if (h >= count) continue;
+      store8(row + (long long)h * D + ln.e0, a);
+      store8(row + (long long)h * D + ln.e1, z);
+    }
+  }
+  if (part == nullptr) return;
+  // the warp's heads (lanes of equal l), then the CTA's warps of each kind, in a fixed order
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = D / 16; o < 32; o <<= 1) {
+      acc0[i] += __shfl_xor_sync(0xffffffffu, acc0[i], o);
+      acc1[i] += __shfl_xor_sync(0xffffffffu, acc1[i], o);
+    }
+    if (ln.sub == 0) {
+      red[warp_id()][ln.e0 + i] = acc0[i];
+      red[warp_id()][ln.e1 + i] = acc1[i];
+    }
+  }
+  if (lane_id() == 0) kinds[warp_id()] = on ? kind : 2;
+  __syncthreads();
+  for (int e = threadIdx.x; e < 2 * D; e += 256) {
+    const int kd = e / D, d = e % D;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+      if (kinds[w] == kd) sum += red[w][d];
+    part[((long long)blockIdx.x * 2 + kd) * D + d] = sum;
+  }
+}
+
+// dq_gain (blockIdx.x 0) and dk_gain (1): 32 columns per CTA, the partial rows of the nparts CTAs added
+// by eight warps, a contiguous eighth each, in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rope_gain_sum(T* __restrict__ dq_gain, T* __restrict__ dk_gain,
+                                                       const float* __restrict__ part, int nparts, int D) {
+  __shared__ float red[8][32];
+  T* out = blockIdx.x == 0 ? dq_gain : dk_gain;
+  if (out == nullptr) return;
+  const int lane = (int)lane_id(), warp = (int)warp_id(), d = (int)blockIdx.y * 32 + lane;
+  const int per = (nparts + 7) / 8, i0 = warp * per, i1 = min(nparts, i0 + per);
+  float s = 0.0f;
+  if (d < D) {
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) s += part[((long long)i * 2 + blockIdx.x) * D + d];
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && d < D) {
+    for (int w = 1; w < 8; ++w) s += red[w][lane];
+    stf(out + d, s);
+  }
+}
+
+// table[t][i] = cos(t theta^(-2i/rot)), table[t][rot/2 + i] = sin of the same angle, in 64 bits:
+// a 32-bit angle at position 131072 would be off by up to 0.008.
+__global__ void k_rope_table(float* __restrict__ table, long long positions, int rot, double theta) {
+  const int half = rot >> 1;
+  const long long n = positions * half;
+  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (long long)gridDim.x * blockDim.x) {
+    const long long t = e / half;
+    const int i = (int)(e - t * half);
+    double s, c;
+    sincos((double)t * pow(theta, -2.0 * (double)i / (double)rot), &s, &c);
+    table[t * rot + i] = (float)c;
+    table[t * rot + half + i] = (float)s;
+  }
+}
+
+}  // namespace beacon

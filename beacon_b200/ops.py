@@ -200,6 +200,178 @@ def attention_bwd_workspace_bytes(B, Hq, S, D, dtype=torch.bfloat16) -> int:
     return int(_lib.lib().beacon_attention_bwd_workspace_size(B, Hq, S, D, _DT[dtype]))
 
 
+# ---------------------------------------------------------------- position rotation, paged cache
+
+def _rows(what, t, width, dtype):
+    """Element stride between the rows of a CUDA matrix of `width` columns whose rows are dense."""
+    if not t.is_cuda or t.dtype != dtype:
+        raise InvalidLaunchConfig(f"{what}: expected a CUDA tensor of {dtype}, got {t.dtype} on {t.device}")
+    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+        raise InvalidLaunchConfig(f"{what}: expected rows of {width} dense elements, got {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+
+
+def _ints(what, t, shape):
+    """A dense int32 CUDA tensor of the given shape (None: not given)."""
+    if t is None:
+        return
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
+        raise InvalidLaunchConfig(f"{what}: expected a contiguous int32 CUDA tensor of shape {tuple(shape)}, "
+                                  f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _rope_args(what, table, q_gain, k_gain, dim, dtype):
+    """(rotated width, table rows) of a rotation table [positions, rot] (None: no rotation)."""
+    for g in (q_gain, k_gain):
+        if g is not None:
+            _dtype(g)
+            if g.dtype != dtype or g.numel() != dim:
+                raise InvalidLaunchConfig(f"{what}: gains must be {dtype} of {dim} elements")
+    if table is None:
+        return 0, 0
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_cuda or not table.is_contiguous():
+        raise InvalidLaunchConfig(f"{what}: the rotation table must be a contiguous float32 CUDA matrix")
+    return table.shape[1], table.shape[0]
+
+
+def _cache(what, k_cache, v_cache, page_table, cu_q, kv_lens):
+    """The paging arguments of the C entry points, from caches [pages, kv_heads, page_size, head_dim]
+    (any strides, the same for both, dense rows) and the sequences' tables."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise InvalidLaunchConfig(f"{what}: caches must be two [pages, kv_heads, page_size, head_dim] of one type")
+    if not k_cache.is_cuda or not v_cache.is_cuda or k_cache.dtype not in _DT:
+        raise InvalidLaunchConfig(f"{what}: caches must be float32 or bfloat16 CUDA tensors")
+    if k_cache.stride() != v_cache.stride() or (k_cache.stride(3) != 1 and k_cache.shape[3] > 1):
+        raise InvalidLaunchConfig(f"{what}: the caches' strides must agree, with dense rows")
+    seqs = kv_lens.numel()
+    _ints(f"{what}: kv_lens", kv_lens, (seqs,))
+    _ints(f"{what}: cu_q", cu_q, (seqs + 1,))
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or page_table.dtype != torch.int32 or \
+            not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise InvalidLaunchConfig(f"{what}: expected an int32 CUDA page table of {seqs} rows")
+    stride = page_table.stride(0) if seqs > 1 else max(page_table.stride(0), page_table.shape[1])
+    pages, _, page_size, _ = k_cache.shape
+    return seqs, (page_table.shape[1], stride, pages, page_size, k_cache.stride(0), k_cache.stride(1),
+                  max(k_cache.stride(2), k_cache.shape[3]) if page_size == 1 else k_cache.stride(2))
+
+
+def rope_table(positions, rot_dim, theta=10000.0, device="cuda"):
+    """float32 [positions, rot_dim]: row t holds cos(t theta^(-2i/rot_dim)), i < rot_dim/2, then the
+    sines.  Made once per model; any table of that layout serves (scaled or extended rotations)."""
+    table = torch.empty(positions, rot_dim, dtype=torch.float32, device=device)
+    check(_lib.lib().beacon_rope_table(_p(table), positions, rot_dim, float(theta), _stream()))
+    return table
+
+
+def qk_norm_rope_fwd(qkv, q_gain, k_gain, table, batch, seq, heads, kv_heads, positions=None, interleaved=False,
+                     eps=1e-5):
+    """(q [B,H,S,D], k [B,Hkv,S,D], v [B,Hkv,S,D]) from qkv [B*S, (H + 2 Hkv) D], the output of the fused
+    QKV projection (query, key, value heads in that order; rows may be strided): per-head RMS norm
+    with gain [D], rotation by the table's row of the token's position (its place in the sequence,
+    or positions [B*S] int32), and the layout attention_fwd reads.  A gain of None: no norm for those
+    heads; table None: no rotation; rotated width below D: the rest of each head passes through."""
+    if heads <= 0 or kv_heads <= 0 or qkv.dim() != 2 or qkv.shape[0] != batch * seq or \
+            qkv.shape[1] % (heads + 2 * kv_heads):
+        raise InvalidLaunchConfig(f"qk_norm_rope_fwd: qkv {tuple(qkv.shape)} is not {batch * seq} rows of "
+                                  f"{heads} + 2 x {kv_heads} heads")
+    D = qkv.shape[1] // (heads + 2 * kv_heads)
+    ld = _rows("qk_norm_rope_fwd: qkv", qkv, qkv.shape[1], qkv.dtype)
+    rot, rows = _rope_args("qk_norm_rope_fwd", table, q_gain, k_gain, D, qkv.dtype)
+    _ints("qk_norm_rope_fwd: positions", positions, (batch * seq,))
+    if qkv.dtype not in _DT:
+        raise InvalidLaunchConfig(f"dtype {qkv.dtype} not supported (float32, bfloat16)")
+    q = torch.empty(batch, heads, seq, D, dtype=qkv.dtype, device=qkv.device)
+    k = torch.empty(batch, kv_heads, seq, D, dtype=qkv.dtype, device=qkv.device)
+    v = torch.empty_like(k)
+    check(_lib.lib().beacon_qk_norm_rope_fwd(_p(q), _p(k), _p(v), _p(qkv), ld, _p(q_gain), _p(k_gain), _p(table), rows,
+                                             _p(positions), batch, seq, heads, kv_heads, D, rot, int(interleaved), eps,
+                                             _DT[qkv.dtype], _stream()))
+    return q, k, v
+
+
+def qk_norm_rope_bwd(dq, dk, dv, qkv, q_gain, k_gain, table, positions=None, interleaved=False, eps=1e-5,
+                     workspace=None):
+    """(dqkv, dq_gain, dk_gain) of qk_norm_rope_fwd for the gradients of its outputs ([B,H,S,D],
+    [B,Hkv,S,D] twice); the norms are formed again from qkv.  A gain of None has no gradient (None)."""
+    if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape:
+        raise InvalidLaunchConfig("qk_norm_rope_bwd: dq [B,H,S,D], dk and dv [B,Hkv,S,D]")
+    B, H, S, D = dq.shape
+    Hkv = dk.shape[1]
+    dt = _dtype(dq, dk, dv)
+    if tuple(dk.shape) != (B, Hkv, S, D) or qkv.shape[0] != B * S:
+        raise InvalidLaunchConfig(f"qk_norm_rope_bwd: dq {tuple(dq.shape)}, dk {tuple(dk.shape)}, "
+                                  f"qkv {tuple(qkv.shape)} do not fit")
+    ld = _rows("qk_norm_rope_bwd: qkv", qkv, (H + 2 * Hkv) * D, dq.dtype)
+    rot, rows = _rope_args("qk_norm_rope_bwd", table, q_gain, k_gain, D, dq.dtype)
+    _ints("qk_norm_rope_bwd: positions", positions, (B * S,))
+    dqkv = torch.empty(B * S, (H + 2 * Hkv) * D, dtype=dq.dtype, device=dq.device)
+    dqg = None if q_gain is None else torch.empty_like(q_gain)
+    dkg = None if k_gain is None else torch.empty_like(k_gain)
+    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    check(_lib.lib().beacon_qk_norm_rope_bwd(_p(dqkv), dqkv.shape[1], _p(dqg), _p(dkg), _p(dq), _p(dk), _p(dv),
+                                             _p(qkv), ld, _p(q_gain), _p(k_gain), _p(table), rows, _p(positions), B, S,
+                                             H, Hkv, D, rot, int(interleaved), eps, dt, ws, wsb, _stream()))
+    return dqkv, dqg, dkg
+
+
+def qk_norm_rope_append(qkv, q_gain, k_gain, table, k_cache, v_cache, page_table, cu_q, kv_lens, heads,
+                        positions=None, interleaved=False, eps=1e-5, q=None):
+    """qk_norm_rope_fwd for new tokens of a batch of sequences: returns the queries [T, H, D] and writes
+    keys and values into the pages of k_cache, v_cache [pages, Hkv, page_size, D] (strided views of a
+    pool serve).  Sequence s owns the rows [cu_q[s], cu_q[s+1]) of qkv [T, (H + 2 Hkv) D] and kv_lens[s]
+    cached tokens with the new ones last; token j of it sits in page page_table[s][j // page_size].  It
+    rotates by j, or by positions [T].  All tables are int32 on the device; nothing is read back."""
+    seqs, paging = _cache("qk_norm_rope_append", k_cache, v_cache, page_table, cu_q, kv_lens)
+    Hkv, D = k_cache.shape[1], k_cache.shape[3]
+    T = qkv.shape[0]
+    ld = _rows("qk_norm_rope_append: qkv", qkv, (heads + 2 * Hkv) * D, k_cache.dtype)
+    rot, rows = _rope_args("qk_norm_rope_append", table, q_gain, k_gain, D, k_cache.dtype)
+    _ints("qk_norm_rope_append: positions", positions, (T,))
+    if q is None:
+        q = torch.empty(T, heads, D, dtype=qkv.dtype, device=qkv.device)
+    elif tuple(q.shape) != (T, heads, D) or q.dtype != qkv.dtype or not q.is_contiguous() or not q.is_cuda:
+        raise InvalidLaunchConfig(f"qk_norm_rope_append: q must be a contiguous {(T, heads, D)} of {qkv.dtype}")
+    check(_lib.lib().beacon_qk_norm_rope_append(_p(q), _p(k_cache), _p(v_cache), _p(qkv), ld, _p(q_gain), _p(k_gain),
+                                                _p(table), rows, _p(positions), _p(cu_q), _p(kv_lens), _p(page_table),
+                                                T, seqs, *paging, heads, Hkv, D, rot, int(interleaved), eps,
+                                                _DT[qkv.dtype], _stream()))
+    return q
+
+
+def paged_attention_workspace_bytes(head_dim, dtype=torch.bfloat16) -> int:
+    return int(_lib.lib().beacon_paged_attention_workspace_size(head_dim, _DT[dtype]))
+
+
+def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q=0, causal=True, out=None, lse=None,
+                    workspace=None):
+    """(out [T, H, D], lse [T, H]): attention of the new tokens q [T, H, D] (dense heads, rows may be
+    strided) over the paged cache; tables as in qk_norm_rope_append, whose call writes the new tokens'
+    keys first.  New token i of a sequence sees the keys up to its own place kv_len - q_len + i (every
+    key with causal=False); a token that sees none gets out 0 and lse -inf.  `max_q`, the largest
+    number of new tokens of a sequence where the caller knows it, only chooses the kernel."""
+    seqs, paging = _cache("paged_attention", k_cache, v_cache, page_table, cu_q, kv_lens)
+    Hkv, D = k_cache.shape[1], k_cache.shape[3]
+    if q.dim() != 3 or q.shape[2] != D or q.dtype != k_cache.dtype or not q.is_cuda:
+        raise InvalidLaunchConfig(f"paged_attention: q {tuple(q.shape)} of {q.dtype} does not fit the cache")
+    T, H, _ = q.shape
+    if T and ((q.stride(2) != 1 and D > 1) or (q.stride(1) != D and H > 1)):
+        raise InvalidLaunchConfig("paged_attention: a token's heads must be dense")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (T, H, D) or out.dtype != q.dtype or not out.is_contiguous() or not out.is_cuda:
+        raise InvalidLaunchConfig(f"paged_attention: out must be a contiguous {(T, H, D)} of {q.dtype}")
+    if lse is None:
+        lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
+    elif tuple(lse.shape) != (T, H) or lse.dtype != torch.float32 or not lse.is_contiguous() or not lse.is_cuda:
+        raise InvalidLaunchConfig(f"paged_attention: lse must be a contiguous float32 {(T, H)}")
+    stride = q.stride(0) if T > 1 else max(q.stride(0), H * D)
+    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    check(_lib.lib().beacon_paged_attention_fwd(_p(out), _p(lse), _p(q), stride, _p(k_cache), _p(v_cache), _p(cu_q),
+                                                _p(kv_lens), _p(page_table), T, seqs, int(max_q or 0), *paging, H, Hkv,
+                                                D, int(causal), _DT[q.dtype], ws, wsb, _stream()))
+    return out, lse
+
+
 # ---------------------------------------------------------------- RMSNorm
 
 def rmsnorm_fwd(x, weight, eps=1e-5):

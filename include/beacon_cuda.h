@@ -327,6 +327,88 @@ int beacon_llama_block_fwd_folded(void* out, const void* x, const void* w_qkv_fo
                                   int64_t head_dim, int64_t d_ff, float eps, int dtype, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* ---- position rotation and paged cache (no reference counterpart) ----------
+ * The reference has no position encoding and no key/value cache; these entries stand between
+ * linear_fwd (the fused QKV projection) and attention in training, and make the block run on new
+ * tokens after earlier ones in serving.
+ *
+ * Rotation table, float32 [positions, rot_dim]: row t holds cos(t theta^(-2i / rot_dim)) for
+ * i < rot_dim / 2, then the sines; evaluated in 64 bits.  Made once; any table of that layout
+ * (scaled or extended rotations) serves the entries below. */
+int beacon_rope_table(float* table, int64_t positions, int64_t rot_dim, double theta, void* stream);
+
+/* Per-head RMS norm of queries and keys, the position rotation and the layout change in one pass.
+ * qkv: batch * seq token rows, qkv_stride elements apart, of q_heads + 2 kv_heads heads of head_dim
+ * (queries, keys, values); q [batch, q_heads, seq, head_dim]; k, v [batch, kv_heads, seq, head_dim]
+ * (v NULL: the value heads are not copied).  For a query or key head x with gain g [head_dim]:
+ *   z = g x / sqrt(mean x^2 + eps)   (gain NULL: z = x, no norm),
+ *   y_a = z_a c_i - z_b s_i,  y_b = z_b c_i + z_a s_i,  y_d = z_d for d >= rot_dim,
+ * (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) when `interleaved`; (c, s) from the table's row of the
+ * token's position: positions [batch * seq], or the place in the sequence when NULL.  rot_dim 0: no
+ * rotation (table may be NULL).  A position outside the table is not followed: the token's query and
+ * key rows are zeros (their gradients too) and the device fault word records code 3.
+ * head_dim up to 256, f32 or bf16 (one rounding, at the store).  16-byte aligned pointers and rows, a
+ * head_dim of 16, 32, 64, 128 or 256 and rot_dim % 16 == 0 take the vectorised kernels. */
+int beacon_qk_norm_rope_fwd(void* q, void* k, void* v, const void* qkv, int64_t qkv_stride, const void* q_gain,
+                            const void* k_gain, const float* table, int64_t table_positions,
+                            const int32_t* positions, int64_t batch, int64_t seq, int64_t q_heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t rot_dim, int interleaved, float eps,
+                            int dtype, void* stream);
+
+/* Its backward, the statistics formed again from qkv (whose value columns are not read):
+ *   dz = the rotation of dy by the opposite angle, dgain = sum over tokens and heads of dz x / r,
+ *   e = g dz, dx = e / r - x sum(e x) / (head_dim r^3)   (dx = dz without a gain).
+ * dqkv rows lie dqkv_stride elements apart; dv NULL leaves their value columns as they are.
+ * dq_gain, dk_gain [head_dim] may be NULL; their sums are kept in float32 and added in a fixed order
+ * (results do not depend on timing).  Workspace as for attention, needed only for gain gradients. */
+int beacon_qk_norm_rope_bwd(void* dqkv, int64_t dqkv_stride, void* dq_gain, void* dk_gain, const void* dq,
+                            const void* dk, const void* dv, const void* qkv, int64_t qkv_stride,
+                            const void* q_gain, const void* k_gain, const float* table, int64_t table_positions,
+                            const int32_t* positions, int64_t batch, int64_t seq, int64_t q_heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t rot_dim, int interleaved, float eps,
+                            int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t beacon_qk_norm_rope_bwd_workspace_size(int64_t head_dim);
+
+/* Paged caches.  k_cache, v_cache: num_pages pages of page_size tokens, any layout with dense rows:
+ * element (page, KV head, token, d) at page * page_stride + head * head_stride + token * token_stride
+ * + d (the same strides for both).  Sequence s of `seqs` owns the token rows [cu_q[s], cu_q[s + 1]) of the
+ * token-major tensors and kv_lens[s] cached tokens, the new ones included and last; its token j
+ * sits in page page_table[s * table_stride + j / page_size] (max_pages entries per row; entries past the
+ * last used page are not read).  cu_q, kv_lens and page_table are int32 in device memory and are read on
+ * the stream: no host copy, so the calls can be captured.  A page index outside the cache is not
+ * followed (its tokens are not written, its keys and values read as zeros), and lengths that reach
+ * past the tensors are cut; both record fault code 3.  Token rows that no sequence owns are ignored.
+ *
+ * qk_norm_rope_append: beacon_qk_norm_rope_fwd for new tokens, the queries written token-major
+ * [tokens, q_heads, head_dim], keys and values into the pages.  Tokens rotate by their place j in the
+ * sequence, or by positions [tokens]. */
+int beacon_qk_norm_rope_append(void* q, void* k_cache, void* v_cache, const void* qkv, int64_t qkv_stride,
+                               const void* q_gain, const void* k_gain, const float* table,
+                               int64_t table_positions, const int32_t* positions, const int32_t* cu_q,
+                               const int32_t* kv_lens, const int32_t* page_table, int64_t tokens, int64_t seqs,
+                               int64_t max_pages, int64_t table_stride, int64_t num_pages, int64_t page_size,
+                               int64_t page_stride, int64_t head_stride, int64_t token_stride, int64_t q_heads,
+                               int64_t kv_heads, int64_t head_dim, int64_t rot_dim, int interleaved, float eps,
+                               int dtype, void* stream);
+
+/* Attention of the new tokens over the cache: q [tokens, q_heads, head_dim] (rows q_stride elements
+ * apart, dense heads), out [tokens, q_heads, head_dim], lse [tokens, q_heads] float32 (may be NULL).  New
+ * token i of a sequence sits at p = kv_len - q_len + i and sees the keys j <= p (causal) or every one:
+ * out = softmax(q k^T / sqrt(head_dim)) v, lse = natural-log logsumexp; a token that sees no key gets out
+ * 0 and lse -inf.  Query head h reads KV head h / (q_heads / kv_heads).  Values in cache slots at or
+ * beyond kv_lens never reach a result, NaN included.  max_q: the largest number of new tokens of a
+ * sequence if known, else 0; it only chooses between kernels.  head_dim 16, 32, 64 or 128; bf16 or f32
+ * (exact fp32 products).  Workspace of beacon_paged_attention_workspace_size bytes, 32-byte aligned
+ * (partial rows of work split along the keys), or NULL for the library's. */
+int beacon_paged_attention_fwd(void* out, float* lse, const void* q, int64_t q_stride, const void* k_cache,
+                               const void* v_cache, const int32_t* cu_q, const int32_t* kv_lens,
+                               const int32_t* page_table, int64_t tokens, int64_t seqs, int64_t max_q,
+                               int64_t max_pages, int64_t table_stride, int64_t num_pages, int64_t page_size,
+                               int64_t page_stride, int64_t head_stride, int64_t token_stride, int64_t q_heads,
+                               int64_t kv_heads, int64_t head_dim, int causal, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+size_t beacon_paged_attention_workspace_size(int64_t head_dim, int dtype);
+
 /* ---- elementwise: crates/beacon-cuda/src/elementwise.rs -------------------- */
 
 /* residual_add (elementwise.rs:47-55): out = a + b */
