@@ -51,14 +51,14 @@ enum : unsigned int {
 
 // Number of i in [1, n] with cu[i] <= t (the sequence that owns token t; n: none does).
 // Whole warp, 32-way: two dependent loads up to 1024 sequences.
-__device__ __forceinline__ int warp_owner(const int* __restrict__ cu, int n, long long t) {
+__device__ __forceinline__ int warp_owner(const int* __restrict__ cu, int n, int t) {
   const int lane = (int)lane_id();
   int lo = 0;
   while (n > 0) {
     const int step = (n + 31) >> 5;
     const bool on = (long long)lane * step < n;
     const int at = min((lane + 1) * step, n);
-    const bool le = on && (long long)__ldg(cu + lo + at) <= t;
+    const bool le = on && __ldg(cu + lo + at) <= t;
     const int c = __popc(__ballot_sync(0xffffffffu, le));
     const int active = __popc(__ballot_sync(0xffffffffu, on));
     const int skip = min(c * step, n);
@@ -68,35 +68,39 @@ __device__ __forceinline__ int warp_owner(const int* __restrict__ cu, int n, lon
   return lo;
 }
 
-// Where a token goes: its rotation row, and the element offset of its slot for KV head 0.
+// Where a token goes: its rotation row, and the element offset of its slot for KV head 0.  32-bit
+// divisions (a token count fits an int): the 64-bit ones were most of the kernels' instructions.
 struct TokenPlace {
-  bool on;          // the token belongs to a sequence (paged form)
-  long long pos;    // table row, -1: none (the head rows are written as zeros)
-  long long slot;   // paged form: cache offset of (page, head 0, token), -1: nowhere
+  bool on;         // the token belongs to a sequence (paged form)
+  int pos;         // table row, -1: none (the head rows are written as zeros)
+  int b, s;        // head-major form: batch entry and place in the sequence
+  long long slot;  // paged form: cache offset of (page, head 0, token), -1: nowhere
 };
 template <bool PAGED>
-__device__ __forceinline__ TokenPlace token_place(const RopeParams& p, long long t) {
-  TokenPlace w{true, 0, -1};
+__device__ __forceinline__ TokenPlace token_place(const RopeParams& p, int t) {
+  TokenPlace w{true, 0, 0, 0, -1};
   if constexpr (PAGED) {
     const PagedSeqs& g = p.pg;
     const int s = warp_owner(g.cu_q, g.seqs, t);
-    if (s >= g.seqs || t < (long long)__ldg(g.cu_q)) {
+    if (s >= g.seqs || t < __ldg(g.cu_q)) {
       w.on = false;
       return w;
     }
-    const long long at = (long long)__ldg(g.kv_lens + s) - ((long long)__ldg(g.cu_q + s + 1) - t);
+    const int at = __ldg(g.kv_lens + s) - (__ldg(g.cu_q + s + 1) - t);
     w.pos = at;
     if (at >= 0) {
-      const long long pi = at / g.page_size;
+      const int pi = (int)((unsigned)at / (unsigned)g.page_size);
       int page = -1;
       if (pi < g.max_pages) page = __ldg(g.page_table + (long long)s * g.table_stride + pi);
       if (page >= 0 && page < g.num_pages)
-        w.slot = (long long)page * g.page_stride + (at - pi * g.page_size) * g.token_stride;
+        w.slot = (long long)page * g.page_stride + (long long)(at - pi * g.page_size) * g.token_stride;
       else if (lane_id() == 0)
         record_fault(kFaultIndex, kSiteRopePage);
     }
   } else {
-    w.pos = t % p.seq;
+    w.b = (int)((unsigned)t / (unsigned)p.seq);
+    w.s = t - w.b * p.seq;
+    w.pos = w.s;
   }
   if (p.positions != nullptr && w.pos >= 0) w.pos = __ldg(p.positions + t);
   if (w.pos < 0 || w.pos >= p.table_positions) {
@@ -106,22 +110,17 @@ __device__ __forceinline__ TokenPlace token_place(const RopeParams& p, long long
   return w;
 }
 
-// Destination of head h (0 .. Hq + 2 Hkv) of token t; null: not written.
+// Destination of head h of kind 0 (query), 1 (key) or 2 (value) of token t; null: not written.
 template <typename T, bool PAGED>
-__device__ __forceinline__ T* head_out(const RopeParams& p, const TokenPlace& w, long long t, int h, T* q, T* k, T* v) {
+__device__ __forceinline__ T* head_out(const RopeParams& p, const TokenPlace& w, int t, int kind, int h, T* q, T* k,
+                                       T* v) {
+  T* base = kind == 0 ? q : kind == 1 ? k : v;
   if constexpr (PAGED) {
-    if (h < p.Hq) return q + (t * p.Hq + h) * p.D;
-    if (w.slot < 0) return nullptr;
-    h -= p.Hq;
-    T* base = h < p.Hkv ? k : v;
-    return base + w.slot + (long long)(h < p.Hkv ? h : h - p.Hkv) * p.pg.head_stride;
+    if (kind == 0) return base + ((long long)t * p.Hq + h) * p.D;
+    return w.slot < 0 ? nullptr : base + w.slot + (long long)h * p.pg.head_stride;
   } else {
-    const long long b = t / p.seq, s = t - b * p.seq;
-    if (h < p.Hq) return q + ((b * p.Hq + h) * p.seq + s) * p.D;
-    h -= p.Hq;
-    T* base = h < p.Hkv ? k : v;
     if (base == nullptr) return nullptr;
-    return base + ((b * p.Hkv + (h < p.Hkv ? h : h - p.Hkv)) * p.seq + s) * p.D;
+    return base + ((long long)(w.b * (kind == 0 ? p.Hq : p.Hkv) + h) * p.seq + w.s) * p.D;
   }
 }
 
@@ -152,23 +151,24 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_any(T* __restrict__ q, T* 
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
     const long long t = u / heads;
     const int h = (int)(u - t * heads);
-    const TokenPlace w = token_place<PAGED>(p, t);
+    const TokenPlace w = token_place<PAGED>(p, (int)t);
     if (!w.on) continue;
-    T* o = head_out<T, PAGED>(p, w, t, h, q, k, v);
+    const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
+    T* o = head_out<T, PAGED>(p, w, (int)t, kind, kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv, q, k, v);
     if (o == nullptr) continue;
     const T* x = qkv + t * p.ld + (long long)h * p.D;
-    if (h >= p.Hq + p.Hkv) {
+    if (kind == 2) {
       for (int d = lane; d < p.D; d += 32) o[d] = x[d];
       continue;
     }
-    const T* g = h < p.Hq ? q_gain : k_gain;
+    const T* g = kind == 0 ? q_gain : k_gain;
     float inv = 1.0f;
     if (g != nullptr) {
       float ss = 0.0f;
       for (int d = lane; d < p.D; d += 32) ss = fmaf(ldf(x + d), ldf(x + d), ss);
       inv = 1.0f / sqrtf(warp_sum(ss) / (float)p.D + p.eps);
     }
-    const float* tab = p.table + w.pos * p.rot;
+    const float* tab = p.table + (long long)w.pos * p.rot;
     for (int d = lane; d < p.D; d += 32) {
       float y = w.pos < 0 ? 0.0f : ldf(x + d) * inv * (g != nullptr ? ldf(g + d) : 1.0f);
       if (w.pos >= 0 && d < p.rot) {
@@ -200,18 +200,19 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
     const long long t = u / heads;
     const int h = (int)(u - t * heads);
-    const TokenPlace w = token_place<false>(p, t);
-    const T* dy = head_out<const T, false>(p, w, t, h, dq, dk, dv);
+    const TokenPlace w = token_place<false>(p, (int)t);
+    const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
+    const T* dy = head_out<const T, false>(p, w, (int)t, kind, kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv, dq,
+                                           dk, dv);
     if (dy == nullptr) continue;
     T* o = dqkv + t * p.ld_out + (long long)h * p.D;
-    if (h >= p.Hq + p.Hkv) {
+    if (kind == 2) {
       for (int d = lane; d < p.D; d += 32) o[d] = dy[d];
       continue;
     }
     const T* x = qkv + t * p.ld + (long long)h * p.D;
-    const int kind = h < p.Hq ? 0 : 1;
     const T* g = kind == 0 ? q_gain : k_gain;
-    const float* tab = p.table + w.pos * p.rot;
+    const float* tab = p.table + (long long)w.pos * p.rot;
     float dz[kRopeMaxDim / 32], ss = 0.0f, ex = 0.0f;
 #pragma unroll
     for (int j = 0; j < kRopeMaxDim / 32; ++j) {
@@ -271,14 +272,51 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
 }
 
 // ---------------------------------------------------------------------------
-// Vectorised forms: head_dim 16 .. 256 (a power of two), rot % 16 == 0, 16-byte aligned rows.
+// Vectorised forms: head_dim 64, 128 or 256, rot % 16 == 0, 16-byte aligned rows.
 //
 // A head takes D/16 lanes, each holding two 8-element chunks rot/2 apart, so that both members of a
 // rotated pair sit in one lane (halves or interleaved) and the only exchange is the sum over the
 // head's lanes; the lanes behind rot/16 hold the pass-through elements the same way.  A warp keeps
 // one batch of U * 32/(D/16) heads of one kind (query, key or value) for every token it visits: its
-// gains stay in registers and a token's cosines and sines are loaded once per batch.
+// gains stay in registers and a token's cosines and sines are loaded once per batch.  Each lane
+// copies its chunks of the next kRopeStages - 1 tokens to shared memory ahead (cp.async; only the
+// lane itself reads them, so nothing synchronises): the bytes in flight do not cost registers.
 // ---------------------------------------------------------------------------
+constexpr int kRopeStages = 3;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A lane's staging area: N chunks of 8 elements per stage, its 16-byte pieces 512 bytes apart (a
+// warp's pieces lie side by side, without bank conflicts).
+template <typename T, int N>
+struct RopeStage {
+  static constexpr int PIECES = (int)sizeof(T) / 2;
+  static constexpr uint32_t BYTES = N * PIECES * 512;  // per warp and stage
+  uint32_t base;
+  __device__ __forceinline__ RopeStage(void* smem, int warp)
+      : base(smem_u32(smem) + warp * kRopeStages * BYTES + lane_id() * 16u) {}
+  __device__ __forceinline__ void fetch(int stage, int chunk, const T* src) const {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      cp_async16(base + stage * BYTES + (chunk * PIECES + k) * 512, reinterpret_cast<const uint4*>(src) + k);
+  }
+  __device__ __forceinline__ void read(int stage, int chunk, Raw8<T>& r) const {
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.u[k].x), "=r"(r.u[k].y), "=r"(r.u[k].z), "=r"(r.u[k].w)
+                   : "r"(base + stage * BYTES + (chunk * PIECES + k) * 512)
+                   : "memory");
+  }
+};
+
 struct RopeBatches {
   int nq, nk;  // batches of query heads, of key heads (value heads: as many as key heads)
   __host__ __device__ int total() const { return nq + 2 * nk; }
@@ -306,7 +344,7 @@ struct RopeLane {
   }
   // Cosines and sines of the lane's eight pairs (1, 0 where nothing turns).  Halves: pair i joins
   // elements i of the two chunks; interleaved: pairs 0-3 lie in the first chunk, 4-7 in the second.
-  __device__ __forceinline__ void turn(const RopeParams& p, long long pos, float (&c)[8], float (&s)[8]) const {
+  __device__ __forceinline__ void turn(const RopeParams& p, int pos, float (&c)[8], float (&s)[8]) const {
     if (!turns || pos < 0) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -315,7 +353,7 @@ struct RopeLane {
       }
       return;
     }
-    const float* tab = p.table + pos * p.rot;
+    const float* tab = p.table + (long long)pos * p.rot;
     const int i0 = p.interleaved ? e0 >> 1 : e0, i1 = p.interleaved ? e1 >> 1 : e0 + 4;
     const int half = p.rot >> 1;
     const float4 c0 = __ldg(reinterpret_cast<const float4*>(tab + i0));
@@ -348,69 +386,89 @@ __device__ __forceinline__ void rope_turn(float (&a)[8], float (&b)[8], const fl
 }
 
 template <typename T>
-__device__ __forceinline__ void ldraw_cs(const T* p, Raw8<T>& r) {  // read once: evict first
-#pragma unroll
-  for (int k = 0; k < (int)(sizeof(T) / 2); ++k) r.u[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
-}
-template <typename T>
 __device__ __forceinline__ void straw(T* p, const Raw8<T>& r) {
 #pragma unroll
   for (int k = 0; k < (int)(sizeof(T) / 2); ++k) reinterpret_cast<uint4*>(p)[k] = r.u[k];
 }
 
+// The warp's batch: kind 0 query, 1 key, 2 value heads; its lane's first head, the kind's count and
+// its first head's column in a token row.
+template <int D, int U>
+struct RopeWork {
+  int kind, h0, count, col, step, t0;
+  bool on;
+  __device__ __forceinline__ RopeWork(const RopeParams& p, const RopeBatches& nb, int sub) {
+    const unsigned n = (unsigned)nb.total(), gw = blockIdx.x * (blockDim.x >> 5) + warp_id();
+    const unsigned warps = gridDim.x * (blockDim.x >> 5);
+    const int b = (int)(gw % n);
+    step = (int)(warps / n);
+    t0 = (int)(gw / n);
+    on = gw < n * (unsigned)step;  // no work for warps beyond a whole number of rounds
+    kind = b < nb.nq ? 0 : b < nb.nq + nb.nk ? 1 : 2;
+    h0 = (kind == 0 ? b : kind == 1 ? b - nb.nq : b - nb.nq - nb.nk) * (U * 32 / (D / 16)) + sub;
+    count = kind == 0 ? p.Hq : p.Hkv;
+    col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
+  }
+};
+
 template <typename T, int D, int U, bool PAGED>
-__global__ void __launch_bounds__(256) k_qk_norm_rope_vec(T* __restrict__ q, T* __restrict__ k, T* __restrict__ v,
-                                                          const T* __restrict__ qkv, const T* __restrict__ q_gain,
-                                                          const T* __restrict__ k_gain, const RopeParams p,
-                                                          const RopeBatches nb) {
+__global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, T* __restrict__ k, T* __restrict__ v,
+                                                             const T* __restrict__ qkv, const T* __restrict__ q_gain,
+                                                             const T* __restrict__ k_gain, const RopeParams p,
+                                                             const RopeBatches nb) {
   constexpr int HPW = 32 / (D / 16);
+  extern __shared__ __align__(16) uint8_t rope_smem[];
   const RopeLane<D> ln(p.rot);
-  const int n = nb.total();
-  const unsigned gw = blockIdx.x * 8u + warp_id(), warps = gridDim.x * 8u;
-  const int b = (int)(gw % (unsigned)n), step = (int)(warps / (unsigned)n);
-  if (gw >= (unsigned)n * (unsigned)step) return;  // warps beyond a whole number of rounds
-  const int kind = b < nb.nq ? 0 : b < nb.nq + nb.nk ? 1 : 2;  // query, key, value heads
-  const int h0 = (kind == 0 ? b : kind == 1 ? b - nb.nq : b - nb.nq - nb.nk) * (U * HPW) + ln.sub;
-  const int count = kind == 0 ? p.Hq : p.Hkv;
-  const int col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
-  const T* gain = kind == 0 ? q_gain : kind == 1 ? k_gain : nullptr;
+  const RopeWork<D, U> w(p, nb, ln.sub);
+  if (!w.on) return;
+  const RopeStage<T, 2 * U> st(rope_smem, (int)warp_id());
+  const T* gain = w.kind == 0 ? q_gain : w.kind == 1 ? k_gain : nullptr;
+  auto fetch = [&](long long t, int stage) {  // 64 bits: t runs past the last token
+    if (t < p.tokens) {
+      const T* row = qkv + t * p.ld + (long long)w.col * D;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = w.h0 + u * HPW;
+        if (h >= w.count) continue;
+        st.fetch(stage, 2 * u, row + (long long)h * D + ln.e0);
+        st.fetch(stage, 2 * u + 1, row + (long long)h * D + ln.e1);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kRopeStages - 1; ++s) fetch(w.t0 + (long long)s * w.step, s);
   Raw8<T> g0, g1;
   if (gain != nullptr) {
     ldraw(gain + ln.e0, g0);
     ldraw(gain + ln.e1, g1);
   }
-  for (long long t = gw / (unsigned)n; t < p.tokens; t += step) {
-    const T* row = qkv + t * p.ld + (long long)col * D;
-    Raw8<T> x0[U], x1[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW;
-      if (h < count) {
-        ldraw_cs(row + (long long)h * D + ln.e0, x0[u]);
-        ldraw_cs(row + (long long)h * D + ln.e1, x1[u]);
-      }
-    }
-    const TokenPlace w = token_place<PAGED>(p, t);
-    if (!w.on) continue;
-    if (kind == 2) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * HPW;
-        T* o = h < count ? head_out<T, PAGED>(p, w, t, col + h, q, k, v) : nullptr;
-        if (o == nullptr) continue;
-        straw(o + ln.e0, x0[u]);
-        straw(o + ln.e1, x1[u]);
-      }
-      continue;
-    }
+  int stage = 0;
+  for (long long t = w.t0; t < p.tokens; t += w.step) {
+    fetch(t + (long long)(kRopeStages - 1) * w.step, stage == 0 ? kRopeStages - 1 : stage - 1);
+    const int at = stage;
+    stage = stage + 1 == kRopeStages ? 0 : stage + 1;
+    const TokenPlace pl = token_place<PAGED>(p, (int)t);
     float c[8], s[8];
-    ln.turn(p, w.pos, c, s);
+    if (w.kind != 2) ln.turn(p, pl.pos, c, s);
+    cp_async_wait<kRopeStages - 1>();
+    if (!pl.on) continue;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW;
+      const int h = w.h0 + u * HPW;
+      T* o = h < w.count ? head_out<T, PAGED>(p, pl, (int)t, w.kind, h, q, k, v) : nullptr;
+      Raw8<T> r0, r1;
+      st.read(at, 2 * u, r0);
+      st.read(at, 2 * u + 1, r1);
+      if (w.kind == 2) {
+        if (o == nullptr) continue;
+        straw(o + ln.e0, r0);
+        straw(o + ln.e1, r1);
+        continue;
+      }
       float a[8], z[8];
-      unraw(x0[u], a);
-      unraw(x1[u], z);
+      unraw(r0, a);
+      unraw(r1, z);
       if (gain != nullptr) {
         float ss = 0.0f;
 #pragma unroll
@@ -426,87 +484,96 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_vec(T* __restrict__ q, T* 
         }
       }
       if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, false);
-      if (w.pos < 0) {
+      if (pl.pos < 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
       }
-      T* o = h < count ? head_out<T, PAGED>(p, w, t, col + h, q, k, v) : nullptr;
       if (o == nullptr) continue;
       store8(o + ln.e0, a);
       store8(o + ln.e1, z);
     }
   }
+  cp_async_wait<0>();
 }
 
 // Backward; part as in k_qk_norm_rope_bwd_any.  A warp keeps the partial sums of its kind's gain
 // gradient for its 16 columns in registers over all its tokens.
 template <typename T, int D, int U>
-__global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_vec(T* __restrict__ dqkv, float* __restrict__ part,
-                                                              const T* __restrict__ dq, const T* __restrict__ dk,
-                                                              const T* __restrict__ dv, const T* __restrict__ qkv,
-                                                              const T* __restrict__ q_gain,
-                                                              const T* __restrict__ k_gain, const RopeParams p,
-                                                              const RopeBatches nb) {
+__global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__ dqkv, float* __restrict__ part,
+                                                                 const T* __restrict__ dq, const T* __restrict__ dk,
+                                                                 const T* __restrict__ dv, const T* __restrict__ qkv,
+                                                                 const T* __restrict__ q_gain,
+                                                                 const T* __restrict__ k_gain, const RopeParams p,
+                                                                 const RopeBatches nb) {
   constexpr int HPW = 32 / (D / 16);
+  extern __shared__ __align__(16) uint8_t rope_smem[];
   __shared__ float red[8][D];
   __shared__ int kinds[8];
   const RopeLane<D> ln(p.rot);
-  const int n = nb.total();
-  const unsigned gw = blockIdx.x * 8u + warp_id(), warps = gridDim.x * 8u;
-  const int b = (int)(gw % (unsigned)n), step = (int)(warps / (unsigned)n);
-  const bool on = gw < (unsigned)n * (unsigned)step;
-  const int kind = b < nb.nq ? 0 : b < nb.nq + nb.nk ? 1 : 2;
-  const int h0 = (kind == 0 ? b : kind == 1 ? b - nb.nq : b - nb.nq - nb.nk) * (U * HPW) + ln.sub;
-  const int count = kind == 0 ? p.Hq : p.Hkv;
-  const int col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
-  const T* gain = kind == 0 ? q_gain : kind == 1 ? k_gain : nullptr;
+  const RopeWork<D, U> w(p, nb, ln.sub);
+  const RopeStage<T, 4 * U> st(rope_smem, (int)warp_id());
+  const T* gain = w.kind == 0 ? q_gain : w.kind == 1 ? k_gain : nullptr;
+  const T* dy = w.kind == 0 ? dq : w.kind == 1 ? dk : dv;
+  const long long last = w.on && dy != nullptr ? p.tokens : 0;
+  auto fetch = [&](long long t, int stage) {
+    if (t < last) {
+      const int b = (int)((unsigned)t / (unsigned)p.seq), sq = (int)t - b * p.seq;
+      const T* y = dy + ((long long)b * w.count * p.seq + sq) * D;
+      const T* x = qkv + t * p.ld + (long long)w.col * D;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = w.h0 + u * HPW;
+        if (h >= w.count) continue;
+        const T* yh = y + (long long)h * p.seq * D;
+        st.fetch(stage, 4 * u, yh + ln.e0);
+        st.fetch(stage, 4 * u + 1, yh + ln.e1);
+        if (gain == nullptr) continue;
+        st.fetch(stage, 4 * u + 2, x + (long long)h * D + ln.e0);
+        st.fetch(stage, 4 * u + 3, x + (long long)h * D + ln.e1);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kRopeStages - 1; ++s) fetch(w.t0 + (long long)s * w.step, s);
   Raw8<T> g0, g1;
   if (gain != nullptr) {
     ldraw(gain + ln.e0, g0);
     ldraw(gain + ln.e1, g1);
   }
   float acc0[8] = {}, acc1[8] = {};
-  for (long long t = on ? gw / (unsigned)n : p.tokens; t < p.tokens; t += step) {
-    const TokenPlace w = token_place<false>(p, t);
-    Raw8<T> y0[U], y1[U], x0[U], x1[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW;
-      if (h >= count) continue;
-      const T* dy = head_out<const T, false>(p, w, t, col + h, dq, dk, dv);
-      if (dy == nullptr) continue;
-      ldraw_cs(dy + ln.e0, y0[u]);
-      ldraw_cs(dy + ln.e1, y1[u]);
-      if (gain != nullptr) {
-        const T* x = qkv + t * p.ld + (long long)(col + h) * D;
-        ldraw_cs(x + ln.e0, x0[u]);
-        ldraw_cs(x + ln.e1, x1[u]);
-      }
-    }
-    T* row = dqkv + t * p.ld_out + (long long)col * D;
-    if (kind == 2) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * HPW;
-        if (h >= count || dv == nullptr) continue;
-        straw(row + (long long)h * D + ln.e0, y0[u]);
-        straw(row + (long long)h * D + ln.e1, y1[u]);
-      }
-      continue;
-    }
+  int stage = 0;
+  for (long long t = w.t0; t < last; t += w.step) {
+    fetch(t + (long long)(kRopeStages - 1) * w.step, stage == 0 ? kRopeStages - 1 : stage - 1);
+    const int at = stage;
+    stage = stage + 1 == kRopeStages ? 0 : stage + 1;
+    const TokenPlace pl = token_place<false>(p, (int)t);
     float c[8], s[8];
-    ln.turn(p, w.pos, c, s);
+    if (w.kind != 2) ln.turn(p, pl.pos, c, s);
+    cp_async_wait<kRopeStages - 1>();
+    T* row = dqkv + t * p.ld_out + (long long)w.col * D;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW;
+      const int h = w.h0 + u * HPW;
+      Raw8<T> r0, r1;
+      st.read(at, 4 * u, r0);
+      st.read(at, 4 * u + 1, r1);
+      if (w.kind == 2) {
+        if (h >= w.count) continue;
+        straw(row + (long long)h * D + ln.e0, r0);
+        straw(row + (long long)h * D + ln.e1, r1);
+        continue;
+      }
       float a[8], z[8];
-      unraw(y0[u], a);
-      unraw(y1[u], z);
+      unraw(r0, a);
+      unraw(r1, z);
       if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, true);
       if (gain != nullptr) {
         float xa[8], xz[8], ga[8], gz[8], ss = 0.0f, ex = 0.0f;
-        unraw(x0[u], xa);
-        unraw(x1[u], xz);
+        st.read(at, 4 * u + 2, r0);
+        st.read(at, 4 * u + 3, r1);
+        unraw(r0, xa);
+        unraw(r1, xz);
         unraw(g0, ga);
         unraw(g1, gz);
 #pragma unroll
@@ -516,26 +583,27 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_vec(T* __restrict__ dq
         }
         const float inv = 1.0f / sqrtf(ln.sum(ss) * (1.0f / D) + p.eps);
         const float back = ln.sum(ex) * inv * inv * (1.0f / D);
-        const float wgt = (h < count && w.pos >= 0) ? inv : 0.0f;
+        const bool counts = h < w.count && pl.pos >= 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (wgt != 0.0f) {
-            acc0[i] = fmaf(a[i] * wgt, xa[i], acc0[i]);
-            acc1[i] = fmaf(z[i] * wgt, xz[i], acc1[i]);
+          if (counts) {
+            acc0[i] = fmaf(a[i] * inv, xa[i], acc0[i]);
+            acc1[i] = fmaf(z[i] * inv, xz[i], acc1[i]);
           }
           a[i] = inv * (a[i] * ga[i] - xa[i] * back);
           z[i] = inv * (z[i] * gz[i] - xz[i] * back);
         }
       }
-      if (w.pos < 0) {
+      if (pl.pos < 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
       }
-      if (h >= count) continue;
+      if (h >= w.count) continue;
       store8(row + (long long)h * D + ln.e0, a);
       store8(row + (long long)h * D + ln.e1, z);
     }
   }
+  cp_async_wait<0>();
   if (part == nullptr) return;
   // the warp's heads (lanes of equal l), then the CTA's warps of each kind, in a fixed order
 #pragma unroll
@@ -550,14 +618,14 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_vec(T* __restrict__ dq
       red[warp_id()][ln.e1 + i] = acc1[i];
     }
   }
-  if (lane_id() == 0) kinds[warp_id()] = on ? kind : 2;
+  if (lane_id() == 0) kinds[warp_id()] = w.on ? w.kind : 2;
   __syncthreads();
   for (int e = threadIdx.x; e < 2 * D; e += 256) {
     const int kd = e / D, d = e % D;
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w)
-      if (kinds[w] == kd) sum += red[w][d];
+    for (int i = 0; i < 8; ++i)
+      if (kinds[i] == kd) sum += red[i][d];
     part[((long long)blockIdx.x * 2 + kd) * D + d] = sum;
   }
 }

@@ -24,7 +24,8 @@ def _p(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the current stream's handle without building a torch Stream object (3.6 us against 0.2)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _dtype(*ts) -> int:
@@ -201,58 +202,65 @@ def attention_bwd_workspace_bytes(B, Hq, S, D, dtype=torch.bfloat16) -> int:
 
 
 # ---------------------------------------------------------------- position rotation, paged cache
+#
+# These are called once or twice per layer and token: each checks its operands in one expression
+# and looks for the reason only when that fails.
 
-def _rows(what, t, width, dtype):
-    """Element stride between the rows of a CUDA matrix of `width` columns whose rows are dense."""
-    if not t.is_cuda or t.dtype != dtype:
-        raise InvalidLaunchConfig(f"{what}: expected a CUDA tensor of {dtype}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
-        raise InvalidLaunchConfig(f"{what}: expected rows of {width} dense elements, got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
-
-
-def _ints(what, t, shape):
-    """A dense int32 CUDA tensor of the given shape (None: not given)."""
-    if t is None:
-        return
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
-        raise InvalidLaunchConfig(f"{what}: expected a contiguous int32 CUDA tensor of shape {tuple(shape)}, "
-                                  f"got {t.dtype} {tuple(t.shape)}")
+def _refuse(what, *tests):
+    """Raise for the first (holds, message) that does not hold."""
+    for holds, message in tests:
+        if not holds:
+            raise InvalidLaunchConfig(f"{what}: {message}")
+    raise InvalidLaunchConfig(f"{what}: operands do not fit")
 
 
-def _rope_args(what, table, q_gain, k_gain, dim, dtype):
-    """(rotated width, table rows) of a rotation table [positions, rot] (None: no rotation)."""
-    for g in (q_gain, k_gain):
-        if g is not None:
-            _dtype(g)
-            if g.dtype != dtype or g.numel() != dim:
-                raise InvalidLaunchConfig(f"{what}: gains must be {dtype} of {dim} elements")
-    if table is None:
-        return 0, 0
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_cuda or not table.is_contiguous():
-        raise InvalidLaunchConfig(f"{what}: the rotation table must be a contiguous float32 CUDA matrix")
-    return table.shape[1], table.shape[0]
+def _dense_i32(t, n):
+    return t.dtype is torch.int32 and t.is_cuda and t.numel() == n and t.is_contiguous()
 
 
-def _cache(what, k_cache, v_cache, page_table, cu_q, kv_lens):
+def _rope_args(what, qkv, width, dim, table, q_gain, k_gain, positions):
+    """(row stride of qkv, rotated width, table rows, dtype code) for token rows of `width` dense elements."""
+    dt, n = qkv.dtype, qkv.shape[0]
+    code = _DT.get(dt)
+    s0, s1 = qkv.stride()
+    table_ok = table is None or (table.dtype is torch.float32 and table.dim() == 2 and table.is_cuda
+                                 and table.is_contiguous())
+    gains_ok = all(g is None or (g.dtype is dt and g.numel() == dim and g.is_cuda and g.is_contiguous())
+                   for g in (q_gain, k_gain))
+    pos_ok = positions is None or _dense_i32(positions, n)
+    if not (code is not None and qkv.is_cuda and qkv.shape[1] == width and (s1 == 1 or width == 1) and table_ok
+            and gains_ok and pos_ok):
+        _refuse(what, (code is not None, f"dtype {dt} not supported (float32, bfloat16)"),
+                (qkv.is_cuda, "operands must be CUDA tensors (no CPU path)"),
+                (qkv.shape[1] == width and s1 == 1, f"qkv must be rows of {width} dense elements, not {tuple(qkv.shape)}"),
+                (table_ok, "the rotation table must be a contiguous float32 CUDA matrix"),
+                (gains_ok, f"gains must be contiguous CUDA tensors of {dim} {dt} elements"),
+                (pos_ok, f"positions must be a contiguous int32 CUDA tensor of {n} elements"))
+    rows, rot = (0, 0) if table is None else table.shape
+    return (s0 if n > 1 else max(s0, width)), rot, rows, code
+
+
+def _paging(what, k_cache, v_cache, page_table, cu_q, kv_lens):
     """The paging arguments of the C entry points, from caches [pages, kv_heads, page_size, head_dim]
-    (any strides, the same for both, dense rows) and the sequences' tables."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-        raise InvalidLaunchConfig(f"{what}: caches must be two [pages, kv_heads, page_size, head_dim] of one type")
-    if not k_cache.is_cuda or not v_cache.is_cuda or k_cache.dtype not in _DT:
-        raise InvalidLaunchConfig(f"{what}: caches must be float32 or bfloat16 CUDA tensors")
-    if k_cache.stride() != v_cache.stride() or (k_cache.stride(3) != 1 and k_cache.shape[3] > 1):
-        raise InvalidLaunchConfig(f"{what}: the caches' strides must agree, with dense rows")
+    (any strides, the same for both, dense rows) and the sequences' tables; ints of the caches' shape."""
+    shape, strides, dt = k_cache.shape, k_cache.stride(), k_cache.dtype
     seqs = kv_lens.numel()
-    _ints(f"{what}: kv_lens", kv_lens, (seqs,))
-    _ints(f"{what}: cu_q", cu_q, (seqs + 1,))
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or page_table.dtype != torch.int32 or \
-            not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
-        raise InvalidLaunchConfig(f"{what}: expected an int32 CUDA page table of {seqs} rows")
-    stride = page_table.stride(0) if seqs > 1 else max(page_table.stride(0), page_table.shape[1])
-    pages, _, page_size, _ = k_cache.shape
-    return seqs, (page_table.shape[1], stride, pages, page_size, k_cache.stride(0), k_cache.stride(1),
-                  max(k_cache.stride(2), k_cache.shape[3]) if page_size == 1 else k_cache.stride(2))
+    if not (len(shape) == 4 and v_cache.shape == shape and v_cache.stride() == strides and v_cache.dtype is dt
+            and k_cache.is_cuda and v_cache.is_cuda and (strides[3] == 1 or shape[3] == 1)
+            and _dense_i32(kv_lens, seqs) and _dense_i32(cu_q, seqs + 1) and page_table.dtype is torch.int32
+            and page_table.is_cuda and page_table.dim() == 2 and page_table.shape[0] == seqs
+            and (page_table.stride(1) == 1 or page_table.shape[1] <= 1)):
+        _refuse(what, (len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is dt,
+                       "caches must be two [pages, kv_heads, page_size, head_dim] of one type"),
+                (k_cache.is_cuda and v_cache.is_cuda, "caches must be CUDA tensors (no CPU path)"),
+                (v_cache.stride() == strides and strides[-1] == 1, "the caches' strides must agree, with dense rows"),
+                (_dense_i32(kv_lens, seqs), "kv_lens must be a contiguous int32 CUDA tensor"),
+                (_dense_i32(cu_q, seqs + 1), f"cu_q must be a contiguous int32 CUDA tensor of {seqs + 1} elements"),
+                (False, f"the page table must be an int32 CUDA matrix of {seqs} rows"))
+    pages, kv_heads, page, dim = shape
+    width = page_table.shape[1]
+    return (seqs, width, page_table.stride(0) if seqs > 1 else max(page_table.stride(0), width), pages, page,
+            strides[0], strides[1], strides[2] if page > 1 else max(strides[2], dim), kv_heads, dim, dt)
 
 
 def rope_table(positions, rot_dim, theta=10000.0, device="cuda"):
@@ -270,22 +278,18 @@ def qk_norm_rope_fwd(qkv, q_gain, k_gain, table, batch, seq, heads, kv_heads, po
     with gain [D], rotation by the table's row of the token's position (its place in the sequence,
     or positions [B*S] int32), and the layout attention_fwd reads.  A gain of None: no norm for those
     heads; table None: no rotation; rotated width below D: the rest of each head passes through."""
-    if heads <= 0 or kv_heads <= 0 or qkv.dim() != 2 or qkv.shape[0] != batch * seq or \
-            qkv.shape[1] % (heads + 2 * kv_heads):
+    n = heads + 2 * kv_heads
+    if heads <= 0 or kv_heads <= 0 or qkv.dim() != 2 or qkv.shape[0] != batch * seq or qkv.shape[1] % n:
         raise InvalidLaunchConfig(f"qk_norm_rope_fwd: qkv {tuple(qkv.shape)} is not {batch * seq} rows of "
                                   f"{heads} + 2 x {kv_heads} heads")
-    D = qkv.shape[1] // (heads + 2 * kv_heads)
-    ld = _rows("qk_norm_rope_fwd: qkv", qkv, qkv.shape[1], qkv.dtype)
-    rot, rows = _rope_args("qk_norm_rope_fwd", table, q_gain, k_gain, D, qkv.dtype)
-    _ints("qk_norm_rope_fwd: positions", positions, (batch * seq,))
-    if qkv.dtype not in _DT:
-        raise InvalidLaunchConfig(f"dtype {qkv.dtype} not supported (float32, bfloat16)")
-    q = torch.empty(batch, heads, seq, D, dtype=qkv.dtype, device=qkv.device)
-    k = torch.empty(batch, kv_heads, seq, D, dtype=qkv.dtype, device=qkv.device)
+    D = qkv.shape[1] // n
+    ld, rot, rows, dt = _rope_args("qk_norm_rope_fwd", qkv, n * D, D, table, q_gain, k_gain, positions)
+    q = torch.empty((batch, heads, seq, D), dtype=qkv.dtype, device=qkv.device)
+    k = torch.empty((batch, kv_heads, seq, D), dtype=qkv.dtype, device=qkv.device)
     v = torch.empty_like(k)
-    check(_lib.lib().beacon_qk_norm_rope_fwd(_p(q), _p(k), _p(v), _p(qkv), ld, _p(q_gain), _p(k_gain), _p(table), rows,
-                                             _p(positions), batch, seq, heads, kv_heads, D, rot, int(interleaved), eps,
-                                             _DT[qkv.dtype], _stream()))
+    check(_lib.lib().beacon_qk_norm_rope_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qkv.data_ptr(), ld, _p(q_gain), _p(k_gain), _p(table), rows,
+        _p(positions), batch, seq, heads, kv_heads, D, rot, int(interleaved), eps, dt, _stream()))
     return q, k, v
 
 
@@ -293,24 +297,26 @@ def qk_norm_rope_bwd(dq, dk, dv, qkv, q_gain, k_gain, table, positions=None, int
                      workspace=None):
     """(dqkv, dq_gain, dk_gain) of qk_norm_rope_fwd for the gradients of its outputs ([B,H,S,D],
     [B,Hkv,S,D] twice); the norms are formed again from qkv.  A gain of None has no gradient (None)."""
-    if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape:
-        raise InvalidLaunchConfig("qk_norm_rope_bwd: dq [B,H,S,D], dk and dv [B,Hkv,S,D]")
+    if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape or qkv.dim() != 2:
+        raise InvalidLaunchConfig("qk_norm_rope_bwd: dq [B,H,S,D], dk and dv [B,Hkv,S,D], qkv [B*S, (H + 2 Hkv) D]")
     B, H, S, D = dq.shape
     Hkv = dk.shape[1]
-    dt = _dtype(dq, dk, dv)
-    if tuple(dk.shape) != (B, Hkv, S, D) or qkv.shape[0] != B * S:
+    if dk.shape != (B, Hkv, S, D) or qkv.shape[0] != B * S:
         raise InvalidLaunchConfig(f"qk_norm_rope_bwd: dq {tuple(dq.shape)}, dk {tuple(dk.shape)}, "
                                   f"qkv {tuple(qkv.shape)} do not fit")
-    ld = _rows("qk_norm_rope_bwd: qkv", qkv, (H + 2 * Hkv) * D, dq.dtype)
-    rot, rows = _rope_args("qk_norm_rope_bwd", table, q_gain, k_gain, D, dq.dtype)
-    _ints("qk_norm_rope_bwd: positions", positions, (B * S,))
-    dqkv = torch.empty(B * S, (H + 2 * Hkv) * D, dtype=dq.dtype, device=dq.device)
+    _dtype(dq, dk, dv)
+    ld, rot, rows, dt = _rope_args("qk_norm_rope_bwd", qkv, (H + 2 * Hkv) * D, D, table, q_gain, k_gain, positions)
+    if qkv.dtype is not dq.dtype:
+        raise InvalidLaunchConfig(f"qk_norm_rope_bwd: mixed dtypes {qkv.dtype} / {dq.dtype}")
+    width = (H + 2 * Hkv) * D
+    dqkv = torch.empty((B * S, width), dtype=dq.dtype, device=dq.device)
     dqg = None if q_gain is None else torch.empty_like(q_gain)
     dkg = None if k_gain is None else torch.empty_like(k_gain)
     ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
-    check(_lib.lib().beacon_qk_norm_rope_bwd(_p(dqkv), dqkv.shape[1], _p(dqg), _p(dkg), _p(dq), _p(dk), _p(dv),
-                                             _p(qkv), ld, _p(q_gain), _p(k_gain), _p(table), rows, _p(positions), B, S,
-                                             H, Hkv, D, rot, int(interleaved), eps, dt, ws, wsb, _stream()))
+    check(_lib.lib().beacon_qk_norm_rope_bwd(
+        dqkv.data_ptr(), width, _p(dqg), _p(dkg), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), ld,
+        _p(q_gain), _p(k_gain), _p(table), rows, _p(positions), B, S, H, Hkv, D, rot, int(interleaved), eps, dt, ws, wsb,
+        _stream()))
     return dqkv, dqg, dkg
 
 
@@ -321,20 +327,19 @@ def qk_norm_rope_append(qkv, q_gain, k_gain, table, k_cache, v_cache, page_table
     pool serve).  Sequence s owns the rows [cu_q[s], cu_q[s+1]) of qkv [T, (H + 2 Hkv) D] and kv_lens[s]
     cached tokens with the new ones last; token j of it sits in page page_table[s][j // page_size].  It
     rotates by j, or by positions [T].  All tables are int32 on the device; nothing is read back."""
-    seqs, paging = _cache("qk_norm_rope_append", k_cache, v_cache, page_table, cu_q, kv_lens)
-    Hkv, D = k_cache.shape[1], k_cache.shape[3]
+    *paging, Hkv, D, dtype = _paging("qk_norm_rope_append", k_cache, v_cache, page_table, cu_q, kv_lens)
+    if qkv.dim() != 2 or qkv.dtype is not dtype:
+        raise InvalidLaunchConfig(f"qk_norm_rope_append: qkv {tuple(qkv.shape)} of {qkv.dtype} beside caches of {dtype}")
     T = qkv.shape[0]
-    ld = _rows("qk_norm_rope_append: qkv", qkv, (heads + 2 * Hkv) * D, k_cache.dtype)
-    rot, rows = _rope_args("qk_norm_rope_append", table, q_gain, k_gain, D, k_cache.dtype)
-    _ints("qk_norm_rope_append: positions", positions, (T,))
+    ld, rot, rows, dt = _rope_args("qk_norm_rope_append", qkv, (heads + 2 * Hkv) * D, D, table, q_gain, k_gain, positions)
     if q is None:
-        q = torch.empty(T, heads, D, dtype=qkv.dtype, device=qkv.device)
-    elif tuple(q.shape) != (T, heads, D) or q.dtype != qkv.dtype or not q.is_contiguous() or not q.is_cuda:
-        raise InvalidLaunchConfig(f"qk_norm_rope_append: q must be a contiguous {(T, heads, D)} of {qkv.dtype}")
-    check(_lib.lib().beacon_qk_norm_rope_append(_p(q), _p(k_cache), _p(v_cache), _p(qkv), ld, _p(q_gain), _p(k_gain),
-                                                _p(table), rows, _p(positions), _p(cu_q), _p(kv_lens), _p(page_table),
-                                                T, seqs, *paging, heads, Hkv, D, rot, int(interleaved), eps,
-                                                _DT[qkv.dtype], _stream()))
+        q = torch.empty((T, heads, D), dtype=dtype, device=qkv.device)
+    elif q.shape != (T, heads, D) or q.dtype is not dtype or not q.is_contiguous() or not q.is_cuda:
+        raise InvalidLaunchConfig(f"qk_norm_rope_append: q must be a contiguous {(T, heads, D)} of {dtype}")
+    check(_lib.lib().beacon_qk_norm_rope_append(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), qkv.data_ptr(), ld, _p(q_gain), _p(k_gain), _p(table), rows,
+        _p(positions), cu_q.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), T, *paging, heads, Hkv, D, rot,
+        int(interleaved), eps, dt, _stream()))
     return q
 
 
@@ -349,26 +354,28 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q=0, cau
     keys first.  New token i of a sequence sees the keys up to its own place kv_len - q_len + i (every
     key with causal=False); a token that sees none gets out 0 and lse -inf.  `max_q`, the largest
     number of new tokens of a sequence where the caller knows it, only chooses the kernel."""
-    seqs, paging = _cache("paged_attention", k_cache, v_cache, page_table, cu_q, kv_lens)
-    Hkv, D = k_cache.shape[1], k_cache.shape[3]
-    if q.dim() != 3 or q.shape[2] != D or q.dtype != k_cache.dtype or not q.is_cuda:
-        raise InvalidLaunchConfig(f"paged_attention: q {tuple(q.shape)} of {q.dtype} does not fit the cache")
+    seqs, *paging, Hkv, D, dtype = _paging("paged_attention", k_cache, v_cache, page_table, cu_q, kv_lens)
+    code = _DT.get(dtype)
+    if q.dim() != 3 or q.shape[2] != D or q.dtype is not dtype or not q.is_cuda or code is None:
+        raise InvalidLaunchConfig(f"paged_attention: q {tuple(q.shape)} of {q.dtype} does not fit the cache "
+                                  f"({dtype}, head_dim {D}; float32 and bfloat16 are supported)")
     T, H, _ = q.shape
-    if T and ((q.stride(2) != 1 and D > 1) or (q.stride(1) != D and H > 1)):
+    s0, s1, s2 = q.stride()
+    if T and ((s2 != 1 and D > 1) or (s1 != D and H > 1)):
         raise InvalidLaunchConfig("paged_attention: a token's heads must be dense")
     if out is None:
-        out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (T, H, D) or out.dtype != q.dtype or not out.is_contiguous() or not out.is_cuda:
-        raise InvalidLaunchConfig(f"paged_attention: out must be a contiguous {(T, H, D)} of {q.dtype}")
+        out = torch.empty((T, H, D), dtype=dtype, device=q.device)
+    elif out.shape != (T, H, D) or out.dtype is not dtype or not out.is_contiguous() or not out.is_cuda:
+        raise InvalidLaunchConfig(f"paged_attention: out must be a contiguous {(T, H, D)} of {dtype}")
     if lse is None:
-        lse = torch.empty(T, H, dtype=torch.float32, device=q.device)
-    elif tuple(lse.shape) != (T, H) or lse.dtype != torch.float32 or not lse.is_contiguous() or not lse.is_cuda:
+        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
+    elif lse.shape != (T, H) or lse.dtype is not torch.float32 or not lse.is_contiguous() or not lse.is_cuda:
         raise InvalidLaunchConfig(f"paged_attention: lse must be a contiguous float32 {(T, H)}")
-    stride = q.stride(0) if T > 1 else max(q.stride(0), H * D)
     ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
-    check(_lib.lib().beacon_paged_attention_fwd(_p(out), _p(lse), _p(q), stride, _p(k_cache), _p(v_cache), _p(cu_q),
-                                                _p(kv_lens), _p(page_table), T, seqs, int(max_q or 0), *paging, H, Hkv,
-                                                D, int(causal), _DT[q.dtype], ws, wsb, _stream()))
+    check(_lib.lib().beacon_paged_attention_fwd(
+        out.data_ptr(), lse.data_ptr(), q.data_ptr(), s0 if T > 1 else max(s0, H * D), k_cache.data_ptr(),
+        v_cache.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), T, seqs, int(max_q or 0), *paging,
+        H, Hkv, D, int(causal), code, ws, wsb, _stream()))
     return out, lse
 
 

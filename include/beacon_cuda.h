@@ -348,7 +348,7 @@ int beacon_rope_table(float* table, int64_t positions, int64_t rot_dim, double t
  * rotation (table may be NULL).  A position outside the table is not followed: the token's query and
  * key rows are zeros (their gradients too) and the device fault word records code 3.
  * head_dim up to 256, f32 or bf16 (one rounding, at the store).  16-byte aligned pointers and rows, a
- * head_dim of 16, 32, 64, 128 or 256 and rot_dim % 16 == 0 take the vectorised kernels. */
+ * head_dim of 64, 128 or 256 and rot_dim % 16 == 0 take the vectorised kernels. */
 int beacon_qk_norm_rope_fwd(void* q, void* k, void* v, const void* qkv, int64_t qkv_stride, const void* q_gain,
                             const void* k_gain, const float* table, int64_t table_positions,
                             const int32_t* positions, int64_t batch, int64_t seq, int64_t q_heads,
