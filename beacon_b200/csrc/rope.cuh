@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
 // copies its chunks of the next kRopeStages - 1 tokens to shared memory ahead (cp.async; only the
 // lane itself reads them, so nothing synchronises): the bytes in flight do not cost registers.
 // ---------------------------------------------------------------------------
-constexpr int kRopeStages = 3;
+constexpr int kRopeStages = 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -314,6 +314,13 @@ struct RopeStage {
                    : "=r"(r.u[k].x), "=r"(r.u[k].y), "=r"(r.u[k].z), "=r"(r.u[k].w)
                    : "r"(base + stage * BYTES + (chunk * PIECES + k) * 512)
                    : "memory");
+  }
+  __device__ __forceinline__ void zero(int chunk, int n) const {
+    for (int s = 0; s < kRopeStages; ++s)
+      for (int k = 0; k < n * PIECES; ++k)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + s * BYTES + (chunk * PIECES + k) * 512),
+                     "r"(0)
+                     : "memory");
   }
 };
 
@@ -365,23 +372,106 @@ struct RopeLane {
   }
 };
 
-// (a, b) = the lane's 16 elements turned by the pairs' angles; `back`: by the opposite angles.
-__device__ __forceinline__ void rope_turn(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8],
-                                          bool interleaved, bool back) {
+// Eight-element arithmetic in f32x2 instructions: issue slots, not bandwidth, are what these kernels run
+// short of (scalar forms measured 2-5% slower).
+__device__ __forceinline__ void mul8(float (&r)[8], const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float sn = back ? -s[i] : s[i];
-    if (interleaved) {
+  for (int i = 0; i < 8; i += 2)
+    mul2(r[i], r[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+}
+__device__ __forceinline__ void scale8(float (&r)[8], const float (&a)[8], float w) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    mul2(r[i], r[i + 1], a[i], a[i + 1], w, w);
+}
+__device__ __forceinline__ void fma8(float (&r)[8], const float (&a)[8], const float (&b)[8], const float (&c)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    fma2(r[i], r[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+}
+__device__ __forceinline__ void fmaw8(float (&r)[8], const float (&a)[8], float w, const float (&c)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    fma2(r[i], r[i + 1], a[i], a[i + 1], w, w, c[i], c[i + 1]);
+}
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8], const float (&c)[8],
+                                      const float (&d)[8]) {
+  float x0 = 0.0f, x1 = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    fma2(x0, x1, a[i], a[i + 1], b[i], b[i + 1], x0, x1);
+    fma2(y0, y1, c[i], c[i + 1], d[i], d[i + 1], y0, y1);
+  }
+  return (x0 + x1) + (y0 + y1);
+}
+
+// A lane's part of a linear map of pairs: element i of the first chunk becomes pa[i] a[i] + qa[i] a'[i], a' its
+// partner (the second chunk's element i, or its neighbour when interleaved); the second chunk likewise.
+struct RopeMap {
+  float pa[8], qa[8], pb[8], qb[8];
+  // rotation by the angles (c, s) after scaling element-wise by (ga, gb)
+  __device__ __forceinline__ void set(const float (&c)[8], const float (&s)[8], const float (&ga)[8],
+                                      const float (&gb)[8], bool interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (interleaved) {
+        const int j = i >> 1;
+        pa[i] = ga[i] * c[j];
+        qa[i] = (i & 1) ? ga[i ^ 1] * s[j] : -ga[i ^ 1] * s[j];
+        pb[i] = gb[i] * c[4 + j];
+        qb[i] = (i & 1) ? gb[i ^ 1] * s[4 + j] : -gb[i ^ 1] * s[4 + j];
+      } else {
+        pa[i] = ga[i] * c[i];
+        qa[i] = -gb[i] * s[i];
+        pb[i] = gb[i] * c[i];
+        qb[i] = ga[i] * s[i];
+      }
+    }
+  }
+  __device__ __forceinline__ void apply(float (&a)[8], float (&b)[8], bool turns, bool interleaved) const {
+    float u[8], w[8];
+    mul8(u, a, pa);
+    mul8(w, b, pb);
+    if (turns) {
+      if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          u[i] = fmaf(a[i ^ 1], qa[i], u[i]);
+          w[i] = fmaf(b[i ^ 1], qb[i], w[i]);
+        }
+      } else {
+        fma8(u, b, qa, u);
+        fma8(w, a, qb, w);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = u[i];
+      b[i] = w[i];
+    }
+  }
+};
+
+// (a, b) = the lane's 16 elements turned back by the pairs' angles.
+__device__ __forceinline__ void rope_back(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8],
+                                          bool interleaved) {
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       float& x = i < 4 ? a[2 * i] : b[2 * i - 8];
       float& y = i < 4 ? a[2 * i + 1] : b[2 * i - 7];
-      const float u = x * c[i] - y * sn, w = y * c[i] + x * sn;
+      const float u = x * c[i] + y * s[i], w = y * c[i] - x * s[i];
       x = u;
       y = w;
-    } else {
-      const float u = a[i] * c[i] - b[i] * sn, w = b[i] * c[i] + a[i] * sn;
-      a[i] = u;
-      b[i] = w;
     }
+  } else {
+    float u[8], w[8], t[8];
+    mul8(u, b, s);
+    mul8(w, a, s);
+    mul8(t, b, c);
+    fma8(a, a, c, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = t[i] - w[i];
   }
 }
 
@@ -410,6 +500,21 @@ struct RopeWork {
     col = kind == 0 ? 0 : kind == 1 ? p.Hq : p.Hq + p.Hkv;
   }
 };
+
+// First element of head 0 of a kind for a token in the output of the forward (or the gradients that
+// the backward reads), and the elements between heads; null: nothing is written.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ T* rope_heads(const RopeParams& p, const TokenPlace& w, int t, int kind, int count, T* base,
+                                         long long& stride) {
+  if constexpr (PAGED) {
+    stride = kind == 0 ? D : p.pg.head_stride;
+    if (kind == 0) return base + (long long)t * p.Hq * D;
+    return w.slot < 0 ? nullptr : base + w.slot;
+  } else {
+    stride = (long long)p.seq * D;
+    return base == nullptr ? nullptr : base + ((long long)w.b * count * p.seq + w.s) * D;
+  }
+}
 
 template <typename T, int D, int U, bool PAGED>
 __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, T* __restrict__ k, T* __restrict__ v,
@@ -449,48 +554,53 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, 
     const int at = stage;
     stage = stage + 1 == kRopeStages ? 0 : stage + 1;
     const TokenPlace pl = token_place<PAGED>(p, (int)t);
-    float c[8], s[8];
-    if (w.kind != 2) ln.turn(p, pl.pos, c, s);
+    RopeMap map;
+    if (w.kind != 2) {
+      float c[8], s[8], ga[8], gz[8];
+      ln.turn(p, pl.pos, c, s);
+      if (gain != nullptr) {
+        unraw(g0, ga);
+        unraw(g1, gz);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ga[i] = gz[i] = 1.0f;
+      }
+      map.set(c, s, ga, gz, p.interleaved != 0);
+    }
+    long long hs;
+    T* const o = rope_heads<T, D, PAGED>(p, pl, (int)t, w.kind, w.count, w.kind == 0 ? q : w.kind == 1 ? k : v, hs);
     cp_async_wait<kRopeStages - 1>();
-    if (!pl.on) continue;
+    if (!pl.on || o == nullptr) continue;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = w.h0 + u * HPW;
-      T* o = h < w.count ? head_out<T, PAGED>(p, pl, (int)t, w.kind, h, q, k, v) : nullptr;
+      T* oh = o + h * hs;
       Raw8<T> r0, r1;
       st.read(at, 2 * u, r0);
       st.read(at, 2 * u + 1, r1);
       if (w.kind == 2) {
-        if (o == nullptr) continue;
-        straw(o + ln.e0, r0);
-        straw(o + ln.e1, r1);
+        if (h < w.count) {
+          straw(oh + ln.e0, r0);
+          straw(oh + ln.e1, r1);
+        }
         continue;
       }
       float a[8], z[8];
       unraw(r0, a);
       unraw(r1, z);
-      if (gain != nullptr) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(z[i], z[i], ss));
-        const float inv = 1.0f / sqrtf(ln.sum(ss) * (1.0f / D) + p.eps);
-        float ga[8], gz[8];
-        unraw(g0, ga);
-        unraw(g1, gz);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] = a[i] * inv * ga[i];
-          z[i] = z[i] * inv * gz[i];
-        }
-      }
-      if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, false);
+      float inv = 1.0f;
+      if (gain != nullptr) inv = rsqrtf(ln.sum(dot8(a, a, z, z)) * (1.0f / D) + p.eps);
+      map.apply(a, z, ln.turns, p.interleaved != 0);
+      if (h >= w.count) continue;
       if (pl.pos < 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
+      } else {
+        scale8(a, a, inv);  // the map is linear: 1/r is applied to the result
+        scale8(z, z, inv);
       }
-      if (o == nullptr) continue;
-      store8(o + ln.e0, a);
-      store8(o + ln.e1, z);
+      store8(oh + ln.e0, a);
+      store8(oh + ln.e1, z);
     }
   }
   cp_async_wait<0>();
@@ -535,6 +645,9 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
     cp_async_commit();
   };
 #pragma unroll
+  for (int u = 0; u < U; ++u)  // heads that the batch lacks read as zeros
+    if (w.h0 + u * HPW >= w.count) st.zero(4 * u, 4);
+#pragma unroll
   for (int s = 0; s < kRopeStages - 1; ++s) fetch(w.t0 + (long long)s * w.step, s);
   Raw8<T> g0, g1;
   if (gain != nullptr) {
@@ -567,34 +680,27 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
       float a[8], z[8];
       unraw(r0, a);
       unraw(r1, z);
-      if (ln.turns) rope_turn(a, z, c, s, p.interleaved != 0, true);
+      if (ln.turns) rope_back(a, z, c, s, p.interleaved != 0);
       if (gain != nullptr) {
-        float xa[8], xz[8], ga[8], gz[8], ss = 0.0f, ex = 0.0f;
+        float xa[8], xz[8], ga[8], gz[8];
         st.read(at, 4 * u + 2, r0);
         st.read(at, 4 * u + 3, r1);
         unraw(r0, xa);
         unraw(r1, xz);
         unraw(g0, ga);
         unraw(g1, gz);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss = fmaf(xa[i], xa[i], fmaf(xz[i], xz[i], ss));
-          ex = fmaf(a[i] * ga[i], xa[i], fmaf(z[i] * gz[i], xz[i], ex));
-        }
-        const float inv = 1.0f / sqrtf(ln.sum(ss) * (1.0f / D) + p.eps);
-        const float back = ln.sum(ex) * inv * inv * (1.0f / D);
-        const bool counts = h < w.count && pl.pos >= 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (counts) {
-            acc0[i] = fmaf(a[i] * inv, xa[i], acc0[i]);
-            acc1[i] = fmaf(z[i] * inv, xz[i], acc1[i]);
-          }
-          a[i] = inv * (a[i] * ga[i] - xa[i] * back);
-          z[i] = inv * (z[i] * gz[i] - xz[i] * back);
-        }
-      }
-      if (pl.pos < 0) {
+        float inv = rsqrtf(ln.sum(dot8(xa, xa, xz, xz)) * (1.0f / D) + p.eps);
+        if (h >= w.count || pl.pos < 0) inv = 0.0f;  // no head, or no position: nothing is added
+        scale8(a, a, inv);  // dz / r
+        scale8(z, z, inv);
+        fma8(acc0, a, xa, acc0);
+        fma8(acc1, z, xz, acc1);
+        mul8(a, a, ga);  // e / r
+        mul8(z, z, gz);
+        const float back = ln.sum(dot8(a, xa, z, xz)) * inv * inv * (-1.0f / D);
+        fmaw8(a, xa, back, a);  // dx = e / r - x sum(e x / r) / (D r^2)
+        fmaw8(z, xz, back, z);
+      } else if (pl.pos < 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
       }
