@@ -29,6 +29,7 @@
 #include "gemm.cuh"
 #include "gemm_fp8.cuh"
 #include "paged.cuh"
+#include "paged_dec.cuh"
 #include "paged_tc.cuh"
 #include "rope.cuh"
 #include "sm100.cuh"

@@ -30,6 +30,7 @@ struct PagedParams {
   long long tokens;
   void* out;                 // [tokens, Hq, D]
   float* lse;                // [tokens, Hq] or null
+  int sched_slot;            // row of g_paged_done
   int4* heads;               // [gridDim.x] the split item that begins in this CTA's run (paged_head)
   float* part_o;             // [2 * gridDim.x, rpi, D]
   float2* part_ml;           // [2 * gridDim.x, rpi] (running maximum, in log2 units; sum)
@@ -39,6 +40,11 @@ enum : unsigned int {
   kSitePagedLens = 0x611,  // cu_q or kv_lens reach past the query rows or the page table
   kSitePagedPage = 0x612,  // a page index outside the cache
 };
+
+// Programmatic dependent launch: the join is launched while the attention kernel runs and waits here
+// for all of its results.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // One contiguous piece of an item: tiles [a, b) of its n.
 struct PagedItem {
@@ -84,7 +90,8 @@ struct PagedWalk {
   int seq, kvh, item, tile;
   int q0, q_len, kv, items;
 
-  __device__ __forceinline__ void start(const PagedParams& p, int kt) {
+  // Run `run` of `runs`.
+  __device__ __forceinline__ void start(const PagedParams& p, int kt, int run, int runs) {
     const int lane = (int)lane_id();
     long long total = 0;
     const long long w0 = paged_seq_work(p, lane, kt);
@@ -92,8 +99,8 @@ struct PagedWalk {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     total *= p.Hkv;
-    chunk = max(1LL, (total + gridDim.x - 1) / gridDim.x);
-    long long at = min((long long)blockIdx.x * chunk, total);
+    chunk = max(1LL, (total + runs - 1) / runs);
+    long long at = min((long long)run * chunk, total);
     left = min(chunk, total - at);
     if (left <= 0) return;
     for (int s0 = 0; s0 < p.pg.seqs; s0 += 32) {
@@ -169,6 +176,41 @@ __device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
 __device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
 
+// The runs that hold pieces of a split item: a run's first piece may continue an item, its last may begin one.
+struct PagedPieces {
+  int first, n;
+  __device__ __forceinline__ long long slot(int i) const { return i == 0 ? 2LL * first + 1 : 2LL * (first + i); }
+};
+__device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x, long long chunk) {
+  // the piece's first tile is at blockIdx.x * chunk when it continues an item; else the item ends x.n - x.b
+  // tiles into the runs that follow
+  if (x.a == 0) return PagedPieces{(int)blockIdx.x, 1 + (int)((x.n - x.b + chunk - 1) / chunk)};
+  const long long begin = (long long)blockIdx.x * chunk - x.a;
+  const int first = (int)(begin / chunk);
+  return PagedPieces{first, (int)((begin + x.n - 1) / chunk) - first + 1};
+}
+
+// Pieces finished per split item (by its first run), one row of counters per launch in flight: the
+// host rotates the rows launch by launch, as it does g_sched's, and the last piece resets its counter.
+constexpr int kPagedMaxRuns = 160;
+__device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns];
+
+// Whole CTA, after its piece has been written: whether every piece of the item now has been.
+__device__ __forceinline__ bool paged_last_piece(const PagedParams& p, const PagedPieces& pc, int* flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned int* done = &g_paged_done[p.sched_slot][pc.first];
+    const bool last = atomicAdd(done, 1u) == (unsigned int)pc.n - 1u;
+    if (last) atomicExch(done, 0u);
+    *flag = last ? 1 : 0;
+  }
+  __syncthreads();
+  const bool last = *flag != 0;
+  if (last) __threadfence();
+  return last;
+}
+
 // Keys that row r (of R) of a piece sees.
 __device__ __forceinline__ int paged_limit(const PagedParams& p, const PagedItem& x, int r) {
   return p.causal ? max(0, x.kv - x.q_len + r / p.g + 1) : x.kv;
@@ -212,9 +254,10 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
   __shared__ int more;
   const int tid = (int)threadIdx.x;
   const int ty = tid >> 4, tx = tid & 15;  // S rows ty + 16 i, keys tx + 16 j; O columns tx + 16 c
+  pdl_launch_dependents();
   PagedWalk walk;
   if (warp_id() == 0) {
-    walk.start(p, KT);
+    walk.start(p, KT, (int)blockIdx.x, (int)gridDim.x);
     if (tid == 0) p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   const int group = p.g;
@@ -354,6 +397,7 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
 // With M = max m: out = sum 2^(m - M) O / sum 2^(m - M) l.
 template <typename T>
 __global__ void __launch_bounds__(128) k_paged_join(const PagedParams p) {
+  pdl_wait();
   const int c = (int)blockIdx.x, lane = (int)lane_id();
   const int4 h = p.heads[c];
   if (h.w == 0) return;

@@ -1,0 +1,308 @@
+// paged_dec.cuh -- attention of few new rows over a paged cache (decode): bf16, head_dim 64 or 128, any
+// page size; definitions and work distribution in paged.cuh.
+//
+// Bound: HBM (each cached key and value is used by the group's rows only, 4 g FLOP per byte).  A
+// 128-row tcgen05 tile would be a few rows full and its chain of S, softmax and PV per 128 keys was
+// what bound it (64 sequences of 500-8192 tokens, 32/8 heads of 128: 170 us against 111 us of HBM
+// time).  Here a CTA's eight warps take the 16-key steps of its run in turn, rows as one 16-row
+// m16n8k16 tile each, and every warp copies its next steps to shared memory ahead (cp.async,
+// kDecStages deep, 192 KB per SM), across item boundaries too.  At an item's end the warps' rows
+// meet in shared memory; the last CTA to finish a split item joins its pieces, in their order.
+#pragma once
+
+#include "paged.cuh"
+
+namespace beacon {
+
+constexpr int kDecStages = 3, kDecWarps = 8, kDecRows = 16, kDecKt = 128;
+template <int D>
+struct PagedDecCfg {
+  static constexpr uint32_t ROW = D * 2;           // bytes of a key
+  static constexpr uint32_t TILE = 16 * ROW;       // 16 keys (or values)
+  static constexpr uint32_t RING = kDecWarps * kDecStages * 2 * TILE;
+  static constexpr int LDO = D + 8;                // merge rows, padded against bank conflicts
+  static constexpr size_t SMEM_BYTES = (size_t)RING + kDecWarps * 8 * LDO * sizeof(float) + kDecWarps * 8 * sizeof(float2);
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8]: thread holds rows lane/4 (c0, c1) and lane/4 + 8 (c2, c3), columns
+// 2 (lane % 4) and the next.
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes, or zeros where `have` is false (nothing is read then).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <int D>
+__global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* __restrict__ q,
+                                                           const __nv_bfloat16* __restrict__ kc,
+                                                           const __nv_bfloat16* __restrict__ vc, const PagedParams p) {
+  using Cfg = PagedDecCfg<D>;
+  constexpr int CH = D / 8;           // 16-byte chunks of a key
+  constexpr int RPL = 32 / CH;        // keys that a warp copies per instruction
+  constexpr int CPL = D / 32;         // columns per lane of a merged row
+  extern __shared__ __align__(128) uint8_t dec_smem[];
+  __shared__ int last_flag;
+  const int lane = (int)lane_id(), warp = (int)warp_id();
+  const uint32_t ring = smem_u32(dec_smem) + warp * kDecStages * 2 * Cfg::TILE;
+  float* mo = reinterpret_cast<float*>(dec_smem + Cfg::RING);                      // [8 warps][8 rows][LDO]
+  float2* mml = reinterpret_cast<float2*>(mo + kDecWarps * 8 * Cfg::LDO);         // [8 warps][8 rows]
+  const float scale_log2 = p.scale * 1.4426950408889634f;
+
+  // fragment addresses within a tile: chunk c of key r lies at chunk c ^ (r & 7) of its row
+  const int kr = (lane & 7) + ((lane >> 4) << 3), kcb = (lane >> 3) & 1;  // K: keys x head dims
+  const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vcb = lane >> 4;  // V, transposed on load
+  const int cr = lane / CH, cc = lane % CH;                               // copies: key cr + RPL i, chunk cc
+
+  PagedWalk walk;  // every warp holds the same
+  walk.start(p, kDecKt, (int)blockIdx.x, (int)gridDim.x);
+  auto steps_of = [](const PagedItem& x) {  // 16-key steps of a piece, at least one
+    const int key0 = x.a * kDecKt;
+    return (min(x.b * kDecKt, max(x.kv, key0 + 1)) - key0 + 15) / 16;
+  };
+
+  // The copies run ahead of the arithmetic on a walk of their own: the warp's next step is step fs of
+  // piece fx, `off` the cache offset of its key (lane & 15), -1 for none.
+  PagedWalk fwalk = walk;
+  PagedItem fx;
+  int fs = 0, fn = 0;
+  bool fon = true;
+  long long off = -1;
+  auto seek = [&]() {
+    while (fon && fs >= fn) {
+      fon = fwalk.next(p, kDecKt, fx);
+      if (fon) {
+        fs = warp;
+        fn = steps_of(fx);
+      }
+    }
+    const int key = fx.a * kDecKt + fs * 16 + (lane & 15);
+    off = fon && key < fx.kv ? paged_key(p.pg, fx.seq, fx.kvh, key) : -1;
+  };
+  int fstage = 0;
+  auto fetch = [&]() {
+    if (fon) {
+      const uint32_t kt = ring + fstage * 2 * Cfg::TILE;
+#pragma unroll
+      for (int i = 0; i < 16 / RPL; ++i) {
+        const int r = cr + RPL * i;
+        const long long o = __shfl_sync(0xffffffffu, off, r);
+        const uint32_t dst = kt + r * Cfg::ROW + ((cc ^ (r & 7)) << 4);
+        const long long e = (o < 0 ? 0 : o) + cc * 8;
+        cp_async16_or_zero(dst, kc + e, o >= 0);
+        cp_async16_or_zero(dst + Cfg::TILE, vc + e, o >= 0);
+      }
+      fs += kDecWarps;
+      seek();
+    }
+    cp_async_commit();
+    fstage = fstage + 1 == kDecStages ? 0 : fstage + 1;
+  };
+  seek();
+#pragma unroll
+  for (int s = 0; s < kDecStages - 1; ++s) fetch();
+
+  // query rows of this thread: lane / 4 and lane / 4 + 8 of the item
+  uint32_t qf[D / 16][4];
+  int lim[2];
+  auto load_q = [&](const PagedItem& x) {
+    const int rows = min(p.rpi, x.q_len * p.g - x.row0);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = lane / 4 + 8 * hf, fr = x.row0 + r;
+      const bool have = r < rows;
+      lim[hf] = have ? min(paged_limit(p, x, fr), x.kv) : 0;
+      const __nv_bfloat16* qr = q + (long long)(x.q0 + (have ? fr / p.g : 0)) * p.q_stride +
+                                ((long long)x.kvh * p.g + (have ? fr % p.g : 0)) * D + 2 * (lane & 3);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        qf[kk][hf] = have ? __ldg(reinterpret_cast<const uint32_t*>(qr + 16 * kk)) : 0u;
+        qf[kk][2 + hf] = have ? __ldg(reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8)) : 0u;
+      }
+    }
+  };
+  // Writes row r of an item (whole) from its sum l relative to the maximum m (log2 units), CPL columns per lane.
+  auto store_row = [&](const PagedItem& x, int r, float m, float l, const float (&o)[CPL]) {
+    const int fr = x.row0 + r;
+    const long long at = (long long)(x.q0 + fr / p.g) * p.Hq + (long long)x.kvh * p.g + fr % p.g;
+    const bool none = m == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / l;
+    uint32_t w[CPL / 2];
+#pragma unroll
+    for (int e = 0; e < CPL; e += 2) w[e / 2] = none ? 0u : pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at * D + CPL * lane);
+    if constexpr (CPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else dst[0] = w[0];
+    if (lane == 0 && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+  };
+
+  PagedItem x;
+  bool more = walk.next(p, kDecKt, x);
+  if (more) load_q(x);
+  int stage = 0;
+  while (more) {
+    float o[D / 8][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const int steps = steps_of(x);
+    for (int s = warp; s < steps; s += kDecWarps) {
+      __syncwarp();  // every lane has read the stage that the next copy overwrites
+      fetch();
+      cp_async_wait<kDecStages - 1>();
+      __syncwarp();
+      const uint32_t kt = ring + stage * 2 * Cfg::TILE, vt = kt + Cfg::TILE;
+      stage = stage + 1 == kDecStages ? 0 : stage + 1;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];
+        ldsm_x4(b, kt + kr * Cfg::ROW + (((2 * kk + kcb) ^ (kr & 7)) << 4));
+        mma_bf16(sc[0], qf[kk], b[0], b[1]);
+        mma_bf16(sc[1], qf[kk], b[2], b[3]);
+      }
+      const int k0 = x.a * kDecKt + s * 16 + 2 * (lane & 3);
+      uint32_t pf[4];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float v[4];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = k0 + 8 * (e >> 1) + (e & 1) < lim[hf] ? sc[e >> 1][2 * hf + (e & 1)] * scale_log2 : -INFINITY;
+          mx = fmaxf(mx, v[e]);
+        }
+        mx = quad_max(mx);
+        const float m_new = fmaxf(m[hf], mx);
+        // as long as the maximum grows by less than 2^8 the old one serves: O, l and P share it
+        const bool need = m_new > m[hf] + 8.0f;
+        if (__any_sync(0xffffffffu, need)) {
+          const float alpha = need ? ex2_approx(m[hf] - m_new) : 1.0f;
+          if (need) m[hf] = m_new;
+          l[hf] *= alpha;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][2 * hf] *= alpha;
+            o[n][2 * hf + 1] *= alpha;
+          }
+        }
+        const float base = m[hf] == -INFINITY ? 0.0f : m[hf];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = ex2_approx(v[e] - base);
+          l[hf] += v[e];
+        }
+        pf[hf] = pack_bf16x2(v[0], v[1]);
+        pf[2 + hf] = pack_bf16x2(v[2], v[3]);
+      }
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t b[4];
+        ldsm_x4_t(b, vt + vr * Cfg::ROW + (((2 * n + vcb) ^ (vr & 7)) << 4));
+        mma_bf16(o[2 * n], pf, b[0], b[1]);
+        mma_bf16(o[2 * n + 1], pf, b[2], b[3]);
+      }
+    }
+    // the next item's query rows load while this one is merged
+    const PagedItem done = x;
+    const int rows = min(p.rpi, done.q_len * p.g - done.row0);
+    more = walk.next(p, kDecKt, x);
+    if (more) load_q(x);
+    const bool whole = done.a == 0 && done.b == done.n;
+    const long long slot = paged_slot(done);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      if (8 * hf >= rows) break;
+      const float ls = quad_sum(l[hf]);
+      float* mr = mo + (warp * 8 + lane / 4) * Cfg::LDO + 2 * (lane & 3);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mr + 8 * n) = make_float2(o[n][2 * hf], o[n][2 * hf + 1]);
+      if ((lane & 3) == 0) mml[warp * 8 + lane / 4] = make_float2(m[hf], ls);
+      __syncthreads();
+      const int r = 8 * hf + warp;
+      if (r < rows) {  // row r: the warps' partial rows in warp order
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, mml[w * 8 + warp].x);
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        float lt = 0.0f, ot[CPL] = {};
+#pragma unroll
+        for (int w = 0; w < kDecWarps; ++w) {
+          const float2 ml = mml[w * 8 + warp];
+          const float wgt = ex2_approx(ml.x - base);
+          lt = fmaf(ml.y, wgt, lt);
+          const float* src = mo + (w * 8 + warp) * Cfg::LDO + CPL * lane;
+#pragma unroll
+          for (int e = 0; e < CPL; ++e) ot[e] = fmaf(src[e], wgt, ot[e]);
+        }
+        if (whole) {
+          store_row(done, r, mx, lt, ot);
+        } else {
+          float* po = p.part_o + (slot * p.rpi + r) * D + CPL * lane;
+#pragma unroll
+          for (int e = 0; e < CPL; ++e) po[e] = ot[e];
+          if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);
+        }
+      }
+      __syncthreads();  // before the buffer is written again
+    }
+    if (whole) continue;
+    // the item's pieces: runs first .. first + pieces - 1
+    const PagedPieces pc = paged_pieces(done, walk.chunk);
+    if (!paged_last_piece(p, pc, &last_flag)) continue;
+    for (int r = warp; r < rows; r += kDecWarps) {
+      float mx = -INFINITY;
+      for (int i = lane; i < pc.n; i += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      const float base = mx == -INFINITY ? 0.0f : mx;
+      float lt = 0.0f, ot[CPL] = {};
+#pragma unroll 4
+      for (int i = 0; i < pc.n; ++i) {
+        const long long at = pc.slot(i) * p.rpi + r;
+        const float2 ml = __ldcg(&p.part_ml[at]);
+        const float wgt = ex2_approx(ml.x - base);
+        lt = fmaf(ml.y, wgt, lt);
+        const float* src = p.part_o + at * D + CPL * lane;
+        if constexpr (CPL == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          ot[0] = fmaf(v.x, wgt, ot[0]);
+          ot[1] = fmaf(v.y, wgt, ot[1]);
+          ot[2] = fmaf(v.z, wgt, ot[2]);
+          ot[3] = fmaf(v.w, wgt, ot[3]);
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          ot[0] = fmaf(v.x, wgt, ot[0]);
+          ot[1] = fmaf(v.y, wgt, ot[1]);
+        }
+      }
+      store_row(done, r, mx, lt, ot);
+    }
+  }
+  cp_async_wait<0>();
+}
+
+}  // namespace beacon

@@ -213,10 +213,11 @@ __global__ void __launch_bounds__(384, 1)
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
+        pdl_launch_dependents();
         p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
       }
       PagedWalk walk;
-      walk.start(p, 128);
+      walk.start(p, 128, (int)blockIdx.x, (int)gridDim.x);
       const int nbox = 128 / tp.box;
       const uint32_t q_tile_bytes = (uint32_t)(tp.tpt * p.g) * 128u * (D / 64);
       uint32_t tk = 0, kissued = 0, vissued = 0, kpar = 0, vpar = 0, qissued = 0, qpar = 0;
