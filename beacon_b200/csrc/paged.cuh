@@ -39,6 +39,7 @@ struct PagedParams {
 enum : unsigned int {
   kSitePagedLens = 0x611,  // cu_q or kv_lens reach past the query rows or the page table
   kSitePagedPage = 0x612,  // a page index outside the cache
+  kSitePagedMerge = 0x613,
 };
 
 // Programmatic dependent launch: the join is launched while the attention kernel runs and waits here
@@ -53,12 +54,18 @@ struct PagedItem {
   int a, b, n;
 };
 
-// Tiles of item i of a sequence.
+// Tiles of item i of a sequence.  The walk is 32-bit arithmetic: the host bounds the number of tiles below
+// 2^31, and the 64-bit divisions cost a decode step more than its loads.
 __device__ __forceinline__ int paged_tiles(int i, int rpi, int g, int q_len, int kv, int causal, int kt) {
-  const long long rows = (long long)q_len * g;
-  const long long last = (min((long long)(i + 1) * rpi, rows) - 1) / g;
-  const long long keys = causal ? max(0LL, (long long)kv - q_len + last + 1) : (long long)kv;
-  return max(1, (int)((keys + kt - 1) / kt));
+  int keys = kv;
+  if (causal) {
+    const unsigned last = (min((unsigned)(i + 1) * (unsigned)rpi, (unsigned)q_len * (unsigned)g) - 1u) / (unsigned)g;
+    keys = max(0, kv - q_len + (int)last + 1);
+  }
+  return max(1, (int)(((unsigned)keys + (unsigned)kt - 1u) / (unsigned)kt));
+}
+__device__ __forceinline__ int paged_items(int q_len, int g, int rpi) {
+  return (int)(((unsigned)q_len * (unsigned)g + (unsigned)rpi - 1u) / (unsigned)rpi);
 }
 // First token, new tokens and cached tokens of sequence s, held inside the tensors that they index.
 __device__ __forceinline__ void paged_lens(const PagedParams& p, int s, int& q0, int& q_len, int& kv) {
@@ -73,61 +80,64 @@ __device__ __forceinline__ void paged_lens(const PagedParams& p, int s, int& q0,
     kv = (int)min((long long)kv, most);
   }
 }
-__device__ __forceinline__ long long paged_seq_work(const PagedParams& p, int s, int kt) {
+__device__ __forceinline__ int paged_seq_work(const PagedParams& p, int s, int kt) {
   if (s >= p.pg.seqs) return 0;
   int q0, q_len, kv;
   paged_lens(p, s, q0, q_len, kv);
-  const int n = (int)(((long long)q_len * p.g + p.rpi - 1) / p.rpi);
-  if (!p.causal) return (long long)n * paged_tiles(0, p.rpi, p.g, q_len, kv, 0, kt);
-  long long w = 0;
+  const int n = paged_items(q_len, p.g, p.rpi);
+  if (n == 0) return 0;
+  if (!p.causal || n == 1) return n * paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt);
+  int w = 0;
   for (int i = 0; i < n; ++i) w += paged_tiles(i, p.rpi, p.g, q_len, kv, 1, kt);
   return w;
 }
 
-// A CTA's run of tiles, walked item by item by one warp (every lane holds the same state).
+// A run of tiles, walked item by item by one warp (every lane holds the same state).
 struct PagedWalk {
-  long long left, chunk;  // tiles left in the run; tiles per run
+  int left, chunk;  // tiles left in the run; tiles per run
   int seq, kvh, item, tile;
   int q0, q_len, kv, items;
 
   // Run `run` of `runs`.
   __device__ __forceinline__ void start(const PagedParams& p, int kt, int run, int runs) {
     const int lane = (int)lane_id();
-    long long total = 0;
-    const long long w0 = paged_seq_work(p, lane, kt);
-    for (int s = lane; s < p.pg.seqs; s += 32) total += (s == lane) ? w0 : paged_seq_work(p, s, kt);
+    const int w0 = paged_seq_work(p, lane, kt);
+    int total = w0;
+#pragma unroll 1
+    for (int s = lane + 32; s < p.pg.seqs; s += 32) total += paged_seq_work(p, s, kt);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     total *= p.Hkv;
-    chunk = max(1LL, (total + runs - 1) / runs);
-    long long at = min((long long)run * chunk, total);
+    chunk = max(1, (int)(((unsigned)total + (unsigned)runs - 1u) / (unsigned)runs));
+    int at = (int)min((unsigned)run * (unsigned)chunk, (unsigned)total);
     left = min(chunk, total - at);
     if (left <= 0) return;
+#pragma unroll 1
     for (int s0 = 0; s0 < p.pg.seqs; s0 += 32) {
-      const long long w = (s0 == 0 ? w0 : paged_seq_work(p, s0 + lane, kt)) * p.Hkv;
-      long long end = w;  // inclusive prefix sum
+      const int per_head = s0 == 0 ? w0 : paged_seq_work(p, s0 + lane, kt);
+      int end = per_head * p.Hkv;  // inclusive prefix sum
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, end, o);
+        const int v = __shfl_up_sync(0xffffffffu, end, o);
         if (lane >= o) end += v;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, at < end);
       if (hit != 0) {
         const int l = __ffs(hit) - 1;
-        const long long seq_work = __shfl_sync(0xffffffffu, w, l);
-        at -= __shfl_sync(0xffffffffu, end, l) - seq_work;
+        const unsigned head_work = (unsigned)__shfl_sync(0xffffffffu, per_head, l);
+        at -= __shfl_sync(0xffffffffu, end, l) - (int)head_work * p.Hkv;
         seq = s0 + l;
         enter(p);
-        const long long per_head = seq_work / p.Hkv;
-        kvh = (int)(at / per_head);
-        at -= kvh * per_head;
+        kvh = (int)((unsigned)at / head_work);
+        at -= kvh * (int)head_work;
         item = 0;
+#pragma unroll 1
         for (int n = paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt); at >= n;
              n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt)) {
           at -= n;
           ++item;
         }
-        tile = (int)at;
+        tile = at;
         return;
       }
       at -= __shfl_sync(0xffffffffu, end, 31);
@@ -136,7 +146,7 @@ struct PagedWalk {
   }
   __device__ __forceinline__ void enter(const PagedParams& p) {
     paged_lens(p, seq, q0, q_len, kv);
-    items = (int)(((long long)q_len * p.g + p.rpi - 1) / p.rpi);
+    items = paged_items(q_len, p.g, p.rpi);
   }
   // The next piece; false at the end of the run.
   __device__ __forceinline__ bool next(const PagedParams& p, int kt, PagedItem& x) {
@@ -149,7 +159,7 @@ struct PagedWalk {
     x.kv = kv;
     x.n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt);
     x.a = tile;
-    x.b = (int)min((long long)x.n, tile + left);
+    x.b = min(x.n, tile + left);
     left -= x.b - x.a;
     tile = 0;
     if (++item >= items) {
@@ -157,6 +167,7 @@ struct PagedWalk {
       if (++kvh >= p.Hkv) {
         kvh = 0;
         if (left > 0) {
+#pragma unroll 1
           do {
             ++seq;
             enter(p);
@@ -170,7 +181,7 @@ struct PagedWalk {
 
 // The split item that begins in a CTA's run, for the join: x = seq, y = KV head, z = item, w = the
 // number of following CTAs that hold the rest of it (0: none begins here).
-__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x, long long chunk) {
+__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x, int chunk) {
   return make_int4(x.seq, x.kvh, x.row0 / p.rpi, (int)((x.n - x.b + chunk - 1) / chunk));
 }
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
@@ -181,34 +192,33 @@ struct PagedPieces {
   int first, n;
   __device__ __forceinline__ long long slot(int i) const { return i == 0 ? 2LL * first + 1 : 2LL * (first + i); }
 };
-__device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x, long long chunk) {
-  // the piece's first tile is at blockIdx.x * chunk when it continues an item; else the item ends x.n - x.b
-  // tiles into the runs that follow
-  if (x.a == 0) return PagedPieces{(int)blockIdx.x, 1 + (int)((x.n - x.b + chunk - 1) / chunk)};
-  const long long begin = (long long)blockIdx.x * chunk - x.a;
-  const int first = (int)(begin / chunk);
-  return PagedPieces{first, (int)((begin + x.n - 1) / chunk) - first + 1};
+__device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x, int chunk) {
+  // a piece that continues an item is its run's first, so the item begins x.a tiles before the run
+  if (x.a == 0) return PagedPieces{(int)blockIdx.x, 1 + (int)((unsigned)(x.n - x.b + chunk - 1) / (unsigned)chunk)};
+  const unsigned begin = blockIdx.x * (unsigned)chunk - (unsigned)x.a;
+  const unsigned first = begin / (unsigned)chunk;
+  return PagedPieces{(int)first, (int)((begin + (unsigned)x.n - 1u) / (unsigned)chunk - first) + 1};
 }
 
-// Pieces finished per split item (by its first run), one row of counters per launch in flight: the
-// host rotates the rows launch by launch, as it does g_sched's, and the last piece resets its counter.
-constexpr int kPagedMaxRuns = 160;
-__device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns];
+// Pieces finished per split item (by its first run) and part of its rows, a set of counters per launch
+// in flight: the host rotates the sets launch by launch, as it does g_sched's slots, and the last
+// piece resets its counter.
+constexpr int kPagedMaxRuns = 160, kPagedParts = 16;
+__device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns][kPagedParts];
 
-// Whole CTA, after its piece has been written: whether every piece of the item now has been.
-__device__ __forceinline__ bool paged_last_piece(const PagedParams& p, const PagedPieces& pc, int* flag) {
+// One warp, after its part of a piece has been written: whether that part of every piece now has been.
+__device__ __forceinline__ bool paged_last_piece(int slot, const PagedPieces& pc, int part) {
   __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned int* done = &g_paged_done[p.sched_slot][pc.first];
-    const bool last = atomicAdd(done, 1u) == (unsigned int)pc.n - 1u;
+  __syncwarp();
+  unsigned int last = 0u;
+  if (lane_id() == 0) {
+    unsigned int* done = &g_paged_done[slot][pc.first][part];
+    last = atomicAdd(done, 1u) == (unsigned int)pc.n - 1u ? 1u : 0u;
     if (last) atomicExch(done, 0u);
-    *flag = last ? 1 : 0;
   }
-  __syncthreads();
-  const bool last = *flag != 0;
+  last = __shfl_sync(0xffffffffu, last, 0);
   if (last) __threadfence();
-  return last;
+  return last != 0u;
 }
 
 // Keys that row r (of R) of a piece sees.

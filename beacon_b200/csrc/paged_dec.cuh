@@ -7,7 +7,8 @@
 // time).  Here a CTA's eight warps take the 16-key steps of its run in turn, rows as one 16-row
 // m16n8k16 tile each, and every warp copies its next steps to shared memory ahead (cp.async,
 // kDecStages deep, 192 KB per SM), across item boundaries too.  At an item's end the warps' rows
-// meet in shared memory; the last CTA to finish a split item joins its pieces, in their order.
+// meet in shared memory, row r merged by warp r % 8 while the others go on; of a split item the warp
+// that writes a row's last piece joins the row's pieces, in their order.
 #pragma once
 
 #include "paged.cuh"
@@ -67,12 +68,21 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   constexpr int RPL = 32 / CH;        // keys that a warp copies per instruction
   constexpr int CPL = D / 32;         // columns per lane of a merged row
   extern __shared__ __align__(128) uint8_t dec_smem[];
-  __shared__ int last_flag;
+  __shared__ uint64_t merge_full, merge_free;  // the merge buffer written, and read, by all eight warps
+  __shared__ int abort_word;
   const int lane = (int)lane_id(), warp = (int)warp_id();
   const uint32_t ring = smem_u32(dec_smem) + warp * kDecStages * 2 * Cfg::TILE;
   float* mo = reinterpret_cast<float*>(dec_smem + Cfg::RING);                      // [8 warps][8 rows][LDO]
   float2* mml = reinterpret_cast<float2*>(mo + kDecWarps * 8 * Cfg::LDO);         // [8 warps][8 rows]
   const float scale_log2 = p.scale * 1.4426950408889634f;
+  volatile int* abort_flag = &abort_word;
+  if (threadIdx.x == 0) {
+    mbar_init(&merge_full, kDecWarps);
+    mbar_init(&merge_free, kDecWarps);
+    abort_word = 0;
+    fence_mbarrier_init();
+  }
+  __syncthreads();
 
   // fragment addresses within a tile: chunk c of key r lies at chunk c ^ (r & 7) of its row
   const int kr = (lane & 7) + ((lane >> 4) << 3), kcb = (lane >> 3) & 1;  // K: keys x head dims
@@ -94,6 +104,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   bool fon = true;
   long long off = -1;
   auto seek = [&]() {
+#pragma unroll 1
     while (fon && fs >= fn) {
       fon = fwalk.next(p, kDecKt, fx);
       if (fon) {
@@ -124,7 +135,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
     fstage = fstage + 1 == kDecStages ? 0 : fstage + 1;
   };
   seek();
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < kDecStages - 1; ++s) fetch();
 
   // query rows of this thread: lane / 4 and lane / 4 + 8 of the item
@@ -162,10 +173,11 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   };
 
   PagedItem x;
-  bool more = walk.next(p, kDecKt, x);
-  if (more) load_q(x);
   int stage = 0;
-  while (more) {
+  uint32_t merges = 0;
+#pragma unroll 1
+  while (walk.next(p, kDecKt, x)) {
+    load_q(x);  // its latency is covered by the copies in flight
     float o[D / 8][4] = {};
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     const int steps = steps_of(x);
@@ -226,29 +238,37 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
         mma_bf16(o[2 * n + 1], pf, b[2], b[3]);
       }
     }
-    // the next item's query rows load while this one is merged
-    const PagedItem done = x;
-    const int rows = min(p.rpi, done.q_len * p.g - done.row0);
-    more = walk.next(p, kDecKt, x);
-    if (more) load_q(x);
-    const bool whole = done.a == 0 && done.b == done.n;
-    const long long slot = paged_slot(done);
+    const int rows = min(p.rpi, x.q_len * p.g - x.row0);
+    const bool whole = x.a == 0 && x.b == x.n;
+    const long long slot = paged_slot(x);
+    const PagedPieces pc = paged_pieces(x, walk.chunk);
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {  // rows r0 .. r0 + 7; the upper eight move down for their turn
+      if (r0 == 8) {
+        m[0] = m[1];
+        l[0] = l[1];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      if (8 * hf >= rows) break;
-      const float ls = quad_sum(l[hf]);
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][0] = o[n][2];
+          o[n][1] = o[n][3];
+        }
+      }
+      const float ls = quad_sum(l[0]);
+      // every warp of the CTA arrives on both barriers for every merge, so these waits end
+      mbar_wait(&merge_free, (merges & 1u) ^ 1u, abort_flag, kSitePagedMerge);
       float* mr = mo + (warp * 8 + lane / 4) * Cfg::LDO + 2 * (lane & 3);
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mr + 8 * n) = make_float2(o[n][2 * hf], o[n][2 * hf + 1]);
-      if ((lane & 3) == 0) mml[warp * 8 + lane / 4] = make_float2(m[hf], ls);
-      __syncthreads();
-      const int r = 8 * hf + warp;
+      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mr + 8 * n) = make_float2(o[n][0], o[n][1]);
+      if ((lane & 3) == 0) mml[warp * 8 + lane / 4] = make_float2(m[0], ls);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge_full);
+      const int r = r0 + warp;
+      float mx = -INFINITY, lt = 0.0f, ot[CPL] = {};
       if (r < rows) {  // row r: the warps' partial rows in warp order
-        float mx = -INFINITY;
+        mbar_wait(&merge_full, merges & 1u, abort_flag, kSitePagedMerge);
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, mml[w * 8 + warp].x);
         const float base = mx == -INFINITY ? 0.0f : mx;
-        float lt = 0.0f, ot[CPL] = {};
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) {
           const float2 ml = mml[w * 8 + warp];
@@ -258,28 +278,28 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
 #pragma unroll
           for (int e = 0; e < CPL; ++e) ot[e] = fmaf(src[e], wgt, ot[e]);
         }
-        if (whole) {
-          store_row(done, r, mx, lt, ot);
-        } else {
-          float* po = p.part_o + (slot * p.rpi + r) * D + CPL * lane;
-#pragma unroll
-          for (int e = 0; e < CPL; ++e) po[e] = ot[e];
-          if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);
-        }
       }
-      __syncthreads();  // before the buffer is written again
-    }
-    if (whole) continue;
-    // the item's pieces: runs first .. first + pieces - 1
-    const PagedPieces pc = paged_pieces(done, walk.chunk);
-    if (!paged_last_piece(p, pc, &last_flag)) continue;
-    for (int r = warp; r < rows; r += kDecWarps) {
-      float mx = -INFINITY;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge_free);
+      ++merges;
+      if (r >= rows) continue;
+      if (whole) {
+        store_row(x, r, mx, lt, ot);
+        continue;
+      }
+      float* po = p.part_o + (slot * p.rpi + r) * D + CPL * lane;
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) po[e] = ot[e];
+      if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);
+      if (!paged_last_piece(p.sched_slot, pc, r)) continue;
+      mx = -INFINITY;
       for (int i = lane; i < pc.n; i += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float base = mx == -INFINITY ? 0.0f : mx;
-      float lt = 0.0f, ot[CPL] = {};
+      lt = 0.0f;
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) ot[e] = 0.0f;
 #pragma unroll 4
       for (int i = 0; i < pc.n; ++i) {
         const long long at = pc.slot(i) * p.rpi + r;
@@ -299,7 +319,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
           ot[1] = fmaf(v.y, wgt, ot[1]);
         }
       }
-      store_row(done, r, mx, lt, ot);
+      store_row(x, r, mx, lt, ot);
     }
   }
   cp_async_wait<0>();
