@@ -12,6 +12,7 @@ import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libbeacon_cuda.so")
+FRONT_PATH = os.path.join(_HERE, "lib", "beacon_front.so")
 CSRC = os.path.join(_HERE, "csrc")
 
 # beacon_status: LaunchError variants (crates/beacon-cuda/src/error.rs:4-13)
@@ -163,6 +164,29 @@ def lib():
                                     ctypes.POINTER(ctypes.c_int64), _sz, _vp])
     _lib = L
     return L
+
+
+_front = None
+
+
+def front():
+    """beacon_front (csrc/front.cpp), bound to the library's entry points: the torch call path of the
+    operators that run once or twice per layer and token."""
+    global _front
+    if _front is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries resolve the module's symbols)
+        if not os.path.exists(FRONT_PATH):
+            raise OSError(f"beacon_front.so not built at {FRONT_PATH}; run beacon_b200._lib.build()")
+        spec = importlib.util.spec_from_file_location("beacon_front", FRONT_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(*(ctypes.cast(getattr(lib(), n), _vp).value for n in (
+            "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd", "beacon_qk_norm_rope_append",
+            "beacon_paged_attention_fwd")))
+        _front = mod
+    return _front
 
 
 def last_error() -> str:

@@ -7,9 +7,10 @@
 // For one KV head the rows are (token, query head of the group), token-major: R = q_len * g.
 //
 // Work: an item is `rpi` consecutive rows of one (sequence, KV head); its length is the number of
-// 128- (or 64-) key tiles its last row sees, at least one.  All items laid end to end (sequence, KV
-// head, item, tile) are cut into gridDim.x equal runs of tiles, one per CTA, so that one long
-// context fills the GPU as well as many short ones and the SMs finish together.  A run's first and
+// 128- (or 64-) key tiles its last row sees, at least one, behind `item_cost` tiles' worth of time for
+// its start and end.  All items laid end to end (sequence, KV head, item, tile) are cut into gridDim.x
+// equal runs, one per CTA, so that one long context fills the GPU as well as many short ones and the
+// SMs finish together.  A run's first and
 // last item may be partial: their unnormalised rows (O, m, l) go to two workspace slots of the CTA
 // and k_paged_join adds them up in tile order, so results do not depend on timing.  Every CTA finds
 // its run itself from cu_q and kv_lens (one warp, 32 sequences per step): no plan, no host copy.
@@ -25,6 +26,7 @@ struct PagedParams {
   int Hq, Hkv, D, g;         // g = Hq / Hkv
   int causal;
   int rpi;                   // rows per item
+  int item_cost;             // time of an item's start and end, in tiles
   float scale;               // 1 / sqrt(D)
   long long q_stride;        // elements between token rows of q
   long long tokens;
@@ -86,21 +88,23 @@ __device__ __forceinline__ int paged_seq_work(const PagedParams& p, int s, int k
   paged_lens(p, s, q0, q_len, kv);
   const int n = paged_items(q_len, p.g, p.rpi);
   if (n == 0) return 0;
-  if (!p.causal || n == 1) return n * paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt);
-  int w = 0;
+  int w = n * p.item_cost;
+  if (!p.causal || n == 1) return w + n * paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt);
   for (int i = 0; i < n; ++i) w += paged_tiles(i, p.rpi, p.g, q_len, kv, 1, kt);
   return w;
 }
 
 // A run of tiles, walked item by item by one warp (every lane holds the same state).
 struct PagedWalk {
-  int left, chunk;  // tiles left in the run; tiles per run
+  int left, chunk;  // tiles left in the run; tiles per run (item costs included)
+  int cost;         // of the next item's start, not yet taken off `left`
   int seq, kvh, item, tile;
   int q0, q_len, kv, items;
 
   // Run `run` of `runs`.
   __device__ __forceinline__ void start(const PagedParams& p, int kt, int run, int runs) {
     const int lane = (int)lane_id();
+    seq = kvh = item = tile = q0 = q_len = kv = items = cost = 0;  // an empty run is never walked
     const int w0 = paged_seq_work(p, lane, kt);
     int total = w0;
 #pragma unroll 1
@@ -132,12 +136,9 @@ struct PagedWalk {
         at -= kvh * (int)head_work;
         item = 0;
 #pragma unroll 1
-        for (int n = paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt); at >= n;
-             n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt)) {
-          at -= n;
-          ++item;
-        }
-        tile = at;
+        for (int n; at >= (n = p.item_cost + paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt)); ++item) at -= n;
+        tile = max(0, at - p.item_cost);
+        cost = max(0, p.item_cost - at);
         return;
       }
       at -= __shfl_sync(0xffffffffu, end, 31);
@@ -150,7 +151,9 @@ struct PagedWalk {
   }
   // The next piece; false at the end of the run.
   __device__ __forceinline__ bool next(const PagedParams& p, int kt, PagedItem& x) {
-    if (left <= 0) return false;
+    left = max(0, left - cost);
+    cost = p.item_cost;
+    if (left == 0) return false;
     x.seq = seq;
     x.kvh = kvh;
     x.row0 = item * p.rpi;
@@ -166,12 +169,14 @@ struct PagedWalk {
       item = 0;
       if (++kvh >= p.Hkv) {
         kvh = 0;
-        if (left > 0) {
+        if (left > cost) {
 #pragma unroll 1
           do {
             ++seq;
             enter(p);
           } while (items == 0 && seq + 1 < p.pg.seqs);  // work is left, so a sequence with tokens follows
+        } else {
+          left = 0;
         }
       }
     }
@@ -179,10 +184,11 @@ struct PagedWalk {
   }
 };
 
-// The split item that begins in a CTA's run, for the join: x = seq, y = KV head, z = item, w = the
-// number of following CTAs that hold the rest of it (0: none begins here).
+// The split item that begins in a CTA's run, for the join: x = the sequence's first token, y = KV head,
+// z = first row, w = pieces << 16 | rows (0: none begins here).
 __device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x, int chunk) {
-  return make_int4(x.seq, x.kvh, x.row0 / p.rpi, (int)((x.n - x.b + chunk - 1) / chunk));
+  const int pieces = 1 + (int)((unsigned)(x.n - x.b + chunk - 1) / (unsigned)chunk);
+  return make_int4(x.q0, x.kvh, x.row0, pieces << 16 | min(p.rpi, x.q_len * p.g - x.row0));
 }
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
 __device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
@@ -402,46 +408,71 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
   }
 }
 
-// Joins split items: CTA (c, y) merges rows y, y + gridDim.y, ... (a warp each) of the item that begins
-// in run c: its piece in slot 2c + 1 and the continuations in slots 2(c + 1), 2(c + 2), ... in order.
-// With M = max m: out = sum 2^(m - M) O / sum 2^(m - M) l.
+// Joins the split items that p.heads lists: all their rows are dealt out to the grid's warps.  The item that
+// begins in run c has its first piece in slot 2c + 1 and the others in slots 2(c + 1), 2(c + 2), .. in
+// order.  With M = max m: out = sum 2^(m - M) O / sum 2^(m - M) l.
+constexpr int kPagedMostRuns = 320;  // of any attention kernel that leaves its joins to this one
 template <typename T>
-__global__ void __launch_bounds__(128) k_paged_join(const PagedParams p) {
+__global__ void __launch_bounds__(512) k_paged_join(const PagedParams p, int runs) {
+  __shared__ int4 heads[kPagedMostRuns];
+  __shared__ int first[kPagedMostRuns + 1];  // rows of the items before
   pdl_wait();
-  const int c = (int)blockIdx.x, lane = (int)lane_id();
-  const int4 h = p.heads[c];
-  if (h.w == 0) return;
-  int q0, q_len, kv;
-  paged_lens(p, h.x, q0, q_len, kv);
-  const int row0 = h.z * p.rpi;
-  const int rows = min(p.rpi, q_len * p.g - row0);
-  for (int r = (int)(blockIdx.y * 4 + warp_id()); r < rows; r += 4 * (int)gridDim.y) {
-    float mx = -INFINITY;
-    for (int i = lane; i <= h.w; i += 32) {
-      const long long slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-      mx = fmaxf(mx, p.part_ml[slot * p.rpi + r].x);
+  const int lane = (int)lane_id();
+  for (int c = (int)threadIdx.x; c < runs; c += 512) heads[c] = p.heads[c];
+  __syncthreads();
+  if (warp_id() == 0) {
+    int sum = 0;
+    for (int c0 = 0; c0 < runs; c0 += 32) {
+      const int rows = c0 + lane < runs ? heads[c0 + lane].w & 0xffff : 0;
+      int end = rows;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+      }
+      if (c0 + lane < runs) first[c0 + lane] = sum + end - rows;
+      sum += __shfl_sync(0xffffffffu, end, 31);
     }
-  #pragma unroll
+    if (lane == 0) first[runs] = sum;
+  }
+  __syncthreads();
+  const int total = first[runs];
+  constexpr int CPL = 4;  // columns per lane
+  const bool on = CPL * lane < p.D;
+  for (int k = (int)(blockIdx.x * 16 + warp_id()); k < total; k += (int)gridDim.x * 16) {
+    int c = 0;
+    for (int step = 256; step > 0; step >>= 1)
+      if (c + step < runs && first[c + step] <= k) c += step;  // the last item that starts at or before row k
+    const int4 h = heads[c];
+    const int r = k - first[c], pieces = h.w >> 16;
+    const PagedPieces pc{c, pieces};
+    float mx = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, p.part_ml[pc.slot(i) * p.rpi + r].x);
+#pragma unroll
     for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
     const float base = mx == -INFINITY ? 0.0f : mx;
-    float l = 0.0f, o[kRopeMaxDim / 32] = {};
-    for (int i = 0; i <= h.w; ++i) {
-      const long long slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-      const float2 ml = p.part_ml[slot * p.rpi + r];
-      if (ml.x == -INFINITY) continue;  // the piece saw no key of this row; its O was not written
+    float l = 0.0f, o[CPL] = {};
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const long long at = pc.slot(i) * p.rpi + r;
+      const float2 ml = p.part_ml[at];
+      const bool have = on && ml.x != -INFINITY;  // a piece without a key of this row has no O
+      const float4 v = have ? *reinterpret_cast<const float4*>(p.part_o + at * p.D + CPL * lane)
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       const float wgt = exp2f(ml.x - base);
       l = fmaf(ml.y, wgt, l);
-      const float* po = p.part_o + (slot * p.rpi + r) * p.D;
-#pragma unroll
-      for (int e = 0; e < kRopeMaxDim / 32; ++e)
-        if (lane + 32 * e < p.D) o[e] = fmaf(po[lane + 32 * e], wgt, o[e]);
+      o[0] = fmaf(v.x, wgt, o[0]);
+      o[1] = fmaf(v.y, wgt, o[1]);
+      o[2] = fmaf(v.z, wgt, o[2]);
+      o[3] = fmaf(v.w, wgt, o[3]);
     }
-    const int fr = row0 + r;
-    const long long at = (long long)(q0 + fr / p.g) * p.Hq + (long long)h.y * p.g + fr % p.g;
+    const int fr = h.z + r;
+    const long long at = (long long)(h.x + fr / p.g) * p.Hq + (long long)h.y * p.g + fr % p.g;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (on) {
 #pragma unroll
-    for (int e = 0; e < kRopeMaxDim / 32; ++e)
-      if (lane + 32 * e < p.D) stf((T*)p.out + at * p.D + lane + 32 * e, o[e] * inv);
+      for (int e = 0; e < CPL; ++e) stf((T*)p.out + at * p.D + CPL * lane + e, o[e] * inv);
+    }
     if (lane == 0 && p.lse != nullptr)
       p.lse[at] = l > 0.0f ? (base + log2f(l)) * 0.69314718055994531f : -INFINITY;
   }

@@ -4,7 +4,7 @@
 // Bound: HBM (each cached key and value is used by the group's rows only, 4 g FLOP per byte).  A
 // 128-row tcgen05 tile would be a few rows full and its chain of S, softmax and PV per 128 keys was
 // what bound it (64 sequences of 500-8192 tokens, 32/8 heads of 128: 170 us against 111 us of HBM
-// time).  Here a CTA's eight warps take the 16-key steps of its run in turn, rows as one 16-row
+// time).  Here a CTA's eight warps take the 16- or 32-key steps of its run in turn, rows as one 16-row
 // m16n8k16 tile each, and every warp copies its next steps to shared memory ahead (cp.async,
 // kDecStages deep, 192 KB per SM), across item boundaries too.  At an item's end the warps' rows
 // meet in shared memory, row r merged by warp r % 8 while the others go on; of a split item the warp
@@ -16,10 +16,13 @@
 namespace beacon {
 
 constexpr int kDecStages = 3, kDecWarps = 8, kDecRows = 16, kDecKt = 128;
+// An item's start and end against 128 keys (90 sequences of 100-1000 tokens: cost 0 59 us, 1 47 us, 2 42 us).
+constexpr int kDecItemCost = 2;
 template <int D>
 struct PagedDecCfg {
+  static constexpr int KS = D == 64 ? 32 : 16;     // keys per step: 8 KB of keys and values
   static constexpr uint32_t ROW = D * 2;           // bytes of a key
-  static constexpr uint32_t TILE = 16 * ROW;       // 16 keys (or values)
+  static constexpr uint32_t TILE = KS * ROW;       // a step's keys (or values)
   static constexpr uint32_t RING = kDecWarps * kDecStages * 2 * TILE;
   static constexpr int LDO = D + 8;                // merge rows, padded against bank conflicts
   static constexpr size_t SMEM_BYTES = (size_t)RING + kDecWarps * 8 * LDO * sizeof(float) + kDecWarps * 8 * sizeof(float2);
@@ -64,6 +67,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
                                                            const __nv_bfloat16* __restrict__ kc,
                                                            const __nv_bfloat16* __restrict__ vc, const PagedParams p) {
   using Cfg = PagedDecCfg<D>;
+  constexpr int KS = Cfg::KS, NT = KS / 8, NH = KS / 16;
   constexpr int CH = D / 8;           // 16-byte chunks of a key
   constexpr int RPL = 32 / CH;        // keys that a warp copies per instruction
   constexpr int CPL = D / 32;         // columns per lane of a merged row
@@ -91,13 +95,13 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
 
   PagedWalk walk;  // every warp holds the same
   walk.start(p, kDecKt, (int)blockIdx.x, (int)gridDim.x);
-  auto steps_of = [](const PagedItem& x) {  // 16-key steps of a piece, at least one
+  auto steps_of = [](const PagedItem& x) {  // steps of a piece, at least one
     const int key0 = x.a * kDecKt;
-    return (min(x.b * kDecKt, max(x.kv, key0 + 1)) - key0 + 15) / 16;
+    return (min(x.b * kDecKt, max(x.kv, key0 + 1)) - key0 + KS - 1) / KS;
   };
 
   // The copies run ahead of the arithmetic on a walk of their own: the warp's next step is step fs of
-  // piece fx, `off` the cache offset of its key (lane & 15), -1 for none.
+  // piece fx, `off` the cache offset of its key (lane % KS), -1 for none.
   PagedWalk fwalk = walk;
   PagedItem fx;
   int fs = 0, fn = 0;
@@ -112,7 +116,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
         fn = steps_of(fx);
       }
     }
-    const int key = fx.a * kDecKt + fs * 16 + (lane & 15);
+    const int key = fx.a * kDecKt + fs * KS + (lane & (KS - 1));
     off = fon && key < fx.kv ? paged_key(p.pg, fx.seq, fx.kvh, key) : -1;
   };
   int fstage = 0;
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
     if (fon) {
       const uint32_t kt = ring + fstage * 2 * Cfg::TILE;
 #pragma unroll
-      for (int i = 0; i < 16 / RPL; ++i) {
+      for (int i = 0; i < KS / RPL; ++i) {
         const int r = cr + RPL * i;
         const long long o = __shfl_sync(0xffffffffu, off, r);
         const uint32_t dst = kt + r * Cfg::ROW + ((cc ^ (r & 7)) << 4);
@@ -188,22 +192,24 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
       __syncwarp();
       const uint32_t kt = ring + stage * 2 * Cfg::TILE, vt = kt + Cfg::TILE;
       stage = stage + 1 == kDecStages ? 0 : stage + 1;
-      float sc[2][4] = {};
+      float sc[NT][4] = {};
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b[4];
-        ldsm_x4(b, kt + kr * Cfg::ROW + (((2 * kk + kcb) ^ (kr & 7)) << 4));
-        mma_bf16(sc[0], qf[kk], b[0], b[1]);
-        mma_bf16(sc[1], qf[kk], b[2], b[3]);
-      }
-      const int k0 = x.a * kDecKt + s * 16 + 2 * (lane & 3);
-      uint32_t pf[4];
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          uint32_t b[4];
+          ldsm_x4(b, kt + (kr + 16 * h) * Cfg::ROW + (((2 * kk + kcb) ^ (kr & 7)) << 4));
+          mma_bf16(sc[2 * h], qf[kk], b[0], b[1]);
+          mma_bf16(sc[2 * h + 1], qf[kk], b[2], b[3]);
+        }
+      const int k0 = x.a * kDecKt + s * KS + 2 * (lane & 3);
+      uint32_t pf[NH][4];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        float v[4];
+        float v[2 * NT];
         float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * NT; ++e) {
           v[e] = k0 + 8 * (e >> 1) + (e & 1) < lim[hf] ? sc[e >> 1][2 * hf + (e & 1)] * scale_log2 : -INFINITY;
           mx = fmaxf(mx, v[e]);
         }
@@ -223,20 +229,25 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
         }
         const float base = m[hf] == -INFINITY ? 0.0f : m[hf];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * NT; ++e) {
           v[e] = ex2_approx(v[e] - base);
           l[hf] += v[e];
         }
-        pf[hf] = pack_bf16x2(v[0], v[1]);
-        pf[2 + hf] = pack_bf16x2(v[2], v[3]);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          pf[h][hf] = pack_bf16x2(v[4 * h], v[4 * h + 1]);
+          pf[h][2 + hf] = pack_bf16x2(v[4 * h + 2], v[4 * h + 3]);
+        }
       }
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];
-        ldsm_x4_t(b, vt + vr * Cfg::ROW + (((2 * n + vcb) ^ (vr & 7)) << 4));
-        mma_bf16(o[2 * n], pf, b[0], b[1]);
-        mma_bf16(o[2 * n + 1], pf, b[2], b[3]);
-      }
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          uint32_t b[4];
+          ldsm_x4_t(b, vt + (vr + 16 * h) * Cfg::ROW + (((2 * n + vcb) ^ (vr & 7)) << 4));
+          mma_bf16(o[2 * n], pf[h], b[0], b[1]);
+          mma_bf16(o[2 * n + 1], pf[h], b[2], b[3]);
+        }
     }
     const int rows = min(p.rpi, x.q_len * p.g - x.row0);
     const bool whole = x.a == 0 && x.b == x.n;
@@ -275,8 +286,11 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
           const float wgt = ex2_approx(ml.x - base);
           lt = fmaf(ml.y, wgt, lt);
           const float* src = mo + (w * 8 + warp) * Cfg::LDO + CPL * lane;
+          float sv[CPL];
+          if constexpr (CPL == 4) *reinterpret_cast<float4*>(sv) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(sv) = *reinterpret_cast<const float2*>(src);
 #pragma unroll
-          for (int e = 0; e < CPL; ++e) ot[e] = fmaf(src[e], wgt, ot[e]);
+          for (int e = 0; e < CPL; ++e) ot[e] = fmaf(sv[e], wgt, ot[e]);
         }
       }
       __syncwarp();

@@ -15,6 +15,12 @@
 //               back into the S region of TMEM, O rescaled there when the maximum grows by over 2^8.
 //               A pair's last key tile may be past tile A's last key: A then ends earlier.
 //
+// An item whose rows fit tile A is `dual`: B takes the same query tile over every other key tile, so
+// that one tile's softmax still runs beside the other's products (a lone tile's chain of S, softmax
+// and PV measured 2.2 us per 128 keys); at its end B's rows go to A through the workspace.  The rows
+// of an item in two pieces are joined by the warp that finishes the second one; k_paged_join joins
+// those of items in more (one warp that reads 16 pieces took 45 us, the whole device a few).
+//
 // TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
 #pragma once
 
@@ -48,9 +54,12 @@ enum : unsigned int {
   kSitePtcO = 0x626,
   kSitePtcClean = 0x627,
   kSitePtcDrain = 0x628,
+  kSitePtcDual = 0x629,
 };
 
 constexpr int kPtcItems = 4;  // items published ahead
+// An item's start and end against a key tile: 1 to 3 measured alike (0: 20% slower at 32-token chunks).
+constexpr int kPtcItemCost = 2;
 struct PtcItem {
   int valid;
   int kvh, tok0;       // KV head; first token row of the item in q
@@ -59,13 +68,20 @@ struct PtcItem {
   int kv;
   int a, b;            // key tiles [a, b)
   int end[2];          // the last key tile + 1 of tiles A, B within [a, b); <= a: none
+  int dual;            // tiles A and B share the query tile and take key tiles a, a+2, .. and a+1, a+3, ..
   int slot;            // workspace slot of a partial piece, -1: the whole item
+  PagedPieces pieces;  // the item's pieces
 };
+// Key tiles of an item's tile t in [a, b): first, step and count.
+__device__ __forceinline__ int ptc_count(const PtcItem& x, int t) {
+  return x.dual ? (x.b - x.a + 1 - t) / 2 : max(0, x.end[t] - x.a);
+}
 
 // 2^a for a pair of arguments on the FMA pipe: a = n + f, f in [-0.5, 0.5], a quartic in f fitted to 2^f by
 // Lawson's iteration on the relative error (2.7e-6 in fp32), n added to the exponent.  The quartic, not
-// the cubic of the training forward, because lse is returned to 1e-5.  Arguments below -126 give less
-// than 2^-125.
+// the cubic of the training forward, because lse is returned to 1e-5.  Arguments below -126, -inf
+// included, give less than 2^-125 instead of 0: masked keys add at most that to a row's sums, and a row
+// that sees no key is known by its maximum.
 __device__ __forceinline__ void exp2_poly4(float& r0, float& r1, float a0, float a1) {
   constexpr float kMagic = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
   a0 = fmaxf(a0, -126.0f);
@@ -84,7 +100,6 @@ __device__ __forceinline__ void exp2_poly4(float& r0, float& r1, float a0, float
 
 // P = 2^(x scale - m) of one 128-key row into the 64 TMEM columns at `taddr` (bf16 pairs); returns the
 // row's sum (fp32, before rounding).  Each 64-key half is handed to the MMA warp once stored.
-template <bool POLY>
 __device__ __forceinline__ float ptc_softmax(const float* x, float scale_log2, float neg_m, uint32_t taddr,
                                              uint64_t* p_half) {
   float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -95,7 +110,7 @@ __device__ __forceinline__ float ptc_softmax(const float* x, float scale_log2, f
     for (int e = 0; e < 32; ++e) {
       float a0, a1, p0, p1;
       fma2(a0, a1, x[64 * c + 2 * e], x[64 * c + 2 * e + 1], scale_log2, scale_log2, neg_m, neg_m);
-      if (POLY && ((kPolyPairs >> (e & 7)) & 1u)) {
+      if ((kPolyPairs >> (e & 7)) & 1u) {
         exp2_poly4(p0, p1, a0, a1);
       } else {
         p0 = ex2_approx(a0);
@@ -157,12 +172,16 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* o_full = p_full + 4;    // [2]
   uint64_t* clean = o_full + 2;     // the MMA warp's lanes have zeroed a V tile's tail
   uint64_t* drain = clean + 1;
-  uint64_t* item_full = drain + 1;               // [kPtcItems]
+  uint64_t* dual_full = drain + 1;               // [4] per 32 rows: B's rows of a dual item are written
+  uint64_t* dual_free = dual_full + 4;           // [4] A has read them
+  uint64_t* item_full = dual_free + 4;           // [kPtcItems]
   uint64_t* item_empty = item_full + kPtcItems;  // [kPtcItems] read by the MMA warp and 8 softmax warps
   PtcItem* items = reinterpret_cast<PtcItem*>(item_empty + kPtcItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPtcItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t warp = warp_id(), lane = lane_id();
+  // rows that B hands to A in dual items: one extra slot per CTA
+  const long long dual_slot = 2LL * gridDim.x + blockIdx.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -181,6 +200,10 @@ __global__ void __launch_bounds__(384, 1)
     }
     mbar_init(clean, 32);
     mbar_init(drain, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&dual_full[i], 1);
+      mbar_init(&dual_free[i], 1);
+    }
     for (int i = 0; i < kPtcItems; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 9);
@@ -237,6 +260,8 @@ __global__ void __launch_bounds__(384, 1)
           x.a = w.a;
           x.b = w.b;
           x.slot = (w.a == 0 && w.b == w.n) ? -1 : paged_slot(w);
+          x.pieces = paged_pieces(w, walk.chunk);
+          x.dual = x.ntok <= tp.tpt ? 1 : 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int last = min((t + 1) * tp.tpt, x.ntok) - 1;
@@ -250,7 +275,7 @@ __global__ void __launch_bounds__(384, 1)
         if (lane == 0) {
           items[is] = x;
           mbar_arrive(&item_full[is]);
-          if (more && w.a == 0 && w.b < w.n) p.heads[blockIdx.x] = paged_head(p, w, walk.chunk);
+          if (more && w.a == 0 && w.b < w.n && x.pieces.n > 2) p.heads[blockIdx.x] = paged_head(p, w, walk.chunk);
         }
         if (!more) break;
         int page = (int)lane < nbox ? ptc_page(p.pg, w.seq, x.a * 128 + (int)lane * tp.box, w.kv) : 0;
@@ -313,8 +338,8 @@ __global__ void __launch_bounds__(384, 1)
       const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
       const uint64_t k_desc = make_sdesc_sw128(smem_u32(sK), 16, 1024);
       const uint64_t v_desc = make_sdesc_sw128(smem_u32(sV), 128 * 128, 1024);
-      auto issue_s = [&](int t, uint32_t k) {
-        const uint64_t qd = sdesc_adv(q_desc, t * Cfg::Q_BYTES), kd = sdesc_adv(k_desc, (k & (ST - 1)) * Cfg::KV_BYTES);
+      auto issue_s = [&](int t, int qt, uint32_t k) {
+        const uint64_t qd = sdesc_adv(q_desc, qt * Cfg::Q_BYTES), kd = sdesc_adv(k_desc, (k & (ST - 1)) * Cfg::KV_BYTES);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
@@ -338,9 +363,18 @@ __global__ void __launch_bounds__(384, 1)
         if (iok) {
           tc_fence_after();
           for (int t = 0; t < 2; ++t)
-            if (x.end[t] > x.a) issue_s(t, tk);
+            if (x.dual ? t == 0 : x.end[t] > x.a) issue_s(t, t, tk);
           if (leader) umma_commit(&k_empty[tk & (ST - 1)]);
           if (n == 1 && leader) umma_commit(q_empty);
+        }
+        if (x.dual && n > 1 && iok) {
+          iok = lane_wait(&k_full[(tk + 1u) & (ST - 1)], ((tk + 1u) >> LOG) & 1u, abort_flag, kSitePtcKv);
+          if (iok) {
+            tc_fence_after();
+            issue_s(1, 0, tk + 1u);
+            if (leader) umma_commit(&k_empty[(tk + 1u) & (ST - 1)]);
+            if (n == 2 && leader) umma_commit(q_empty);
+          }
         }
         for (int i = 0; i < n && iok; ++i) {
           const int j = x.a + i;
@@ -361,9 +395,10 @@ __global__ void __launch_bounds__(384, 1)
           }
           const uint64_t vd = sdesc_adv(v_desc, (tv & (ST - 1)) * Cfg::KV_BYTES);
           for (int t = 0; t < 2 && iok; ++t) {
-            if (j >= x.end[t]) continue;
+            if (x.dual ? t != (i & 1) : j >= x.end[t]) continue;
+            const uint32_t it = (uint32_t)(x.dual ? i >> 1 : i);  // the tile's how manieth key tile
             for (int hf = 0; hf < 2 && iok; ++hf) {
-              if (!lane_wait(&p_full[2 * t + hf], (ns[t] + (uint32_t)i) & 1u, abort_flag, kSitePtcP)) {
+              if (!lane_wait(&p_full[2 * t + hf], (ns[t] + it) & 1u, abort_flag, kSitePtcP)) {
                 iok = false;
                 break;
               }
@@ -373,10 +408,22 @@ __global__ void __launch_bounds__(384, 1)
                 const int kk = 4 * hf + k4;
                 if (leader)
                   umma_f16_ts(tmem + 256 + t * D, tmem + 128 * t + kk * 8, sdesc_adv(vd, kk * 2048), idesc_o,
-                              (i > 0 || kk > 0) ? 1u : 0u);
+                              (it > 0 || kk > 0) ? 1u : 0u);
               }
             }
             if (!iok) break;
+            if (x.dual) {
+              if (i + 2 >= n && leader) umma_commit(&o_full[t]);
+              if (i + 2 < n) {
+                const uint32_t t2 = tv + 2u;
+                if (!lane_wait(&k_full[t2 & (ST - 1)], (t2 >> LOG) & 1u, abort_flag, kSitePtcKv)) { iok = false; break; }
+                tc_fence_after();
+                issue_s(t, 0, t2);
+                if (leader) umma_commit(&k_empty[t2 & (ST - 1)]);
+                if (i + 3 == n && leader) umma_commit(q_empty);
+              }
+              continue;
+            }
             if (j == x.end[t] - 1 && leader) umma_commit(&o_full[t]);
             if (j + 1 < x.end[t]) {
               if (!k_next) {
@@ -384,17 +431,17 @@ __global__ void __launch_bounds__(384, 1)
                 tc_fence_after();
                 k_next = true;
               }
-              issue_s(t, tn);
+              issue_s(t, t, tn);
             }
           }
           if (!iok) break;
           if (leader) umma_commit(&v_empty[tv & (ST - 1)]);
           if (k_next && leader) umma_commit(&k_empty[tn & (ST - 1)]);
-          if (i + 2 == n && leader) umma_commit(q_empty);
+          if (!x.dual && i + 2 == n && leader) umma_commit(q_empty);
         }
         ok = iok;
         tk += (uint32_t)n;
-        for (int t = 0; t < 2; ++t) ns[t] += (uint32_t)max(0, x.end[t] - x.a);
+        for (int t = 0; t < 2; ++t) ns[t] += (uint32_t)ptc_count(x, t);
         __syncwarp();
         if (ok && leader) mbar_arrive(&item_empty[ci % kPtcItems]);
       }
@@ -412,36 +459,46 @@ __global__ void __launch_bounds__(384, 1)
     const int rt = r / p.g;  // token of the tile
     const bool in_tile = rt < tp.tpt;
     const int head = r - rt * p.g;
-    uint32_t ns = 0, no = 0;
+    uint32_t ns = 0, no = 0, duals = 0;
     bool ok = true;
     for (int ci = 0; ok; ++ci) {
       PtcItem x;
       const bool more = __all_sync(0xffffffffu, read_item(ci, x));
       if (lane == 0) mbar_arrive(&item_empty[ci % kPtcItems]);
       if (!more) break;
-      const int end = x.end[t], tok = t * tp.tpt + rt;
+      const int count = ptc_count(x, t), tok = (x.dual ? 0 : t * tp.tpt) + rt;
       const bool row_ok = in_tile && tok < x.ntok;
       // rows that are stored nowhere count as seeing every key, so that they do not force the masked path
       const int lim = !row_ok ? INT32_MAX : p.causal ? max(0, x.lim0 + tok) : x.kv;
       float m_used = -INFINITY, l = 0.0f;
-      for (int j = x.a; j < end; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (ns + (uint32_t)(j - x.a)) & 1u, abort_flag, kSitePtcS))) {
+      for (int i = 0; i < count; ++i) {
+        const int j = x.dual ? x.a + t + 2 * i : x.a + i;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], (ns + (uint32_t)i) & 1u, abort_flag, kSitePtcS))) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const int limit = lim - j * 128;
+        if (!__all_sync(0xffffffffu, limit >= 128)) {
+          // keys past the row's limit become -inf in TMEM, so that one softmax serves every tile: a second
+          // one for masked tiles cost ~6k cycles of instruction fetch at its first use in a launch
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t u[32];
+            tmem_ld32(tmem + lane_base + s_col + c, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) u[e] = c + e < limit ? u[e] : 0xff800000u;
+            tmem_st32(tmem + lane_base + s_col + c, u);
+          }
+          tmem_wait_st();
+        }
         uint32_t xu[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           tmem_ld32(tmem + lane_base + s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&xu[32 * c]));
         tmem_wait_ld();
         float* xs = reinterpret_cast<float*>(xu);
-        const int limit = lim - j * 128;
-        const bool unmasked = __all_sync(0xffffffffu, limit >= 128);
-        if (!unmasked) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) xs[c] = (c < limit) ? xs[c] : -INFINITY;
-        }
         float m8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) m8[u] = fmaxf(xs[u], xs[8 + u]);
@@ -452,7 +509,7 @@ __global__ void __launch_bounds__(384, 1)
         const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
                          tp.scale_log2;
         const float m_new = fmaxf(m_used, mx);
-        if (j == x.a) {
+        if (i == 0) {
           m_used = m_new;
         } else {
           // a row without a key so far has O = 0 and m = -inf: 2^(-inf) = 0 rescales it
@@ -475,67 +532,167 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
         const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
-        if (unmasked)
-          l += ptc_softmax<true>(xs, tp.scale_log2, neg_m, tmem + lane_base + s_col, &p_full[2 * t]);
-        else
-          l += ptc_softmax<false>(xs, tp.scale_log2, neg_m, tmem + lane_base + s_col, &p_full[2 * t]);
+        l += ptc_softmax(xs, tp.scale_log2, neg_m, tmem + lane_base + s_col, &p_full[2 * t]);
       }
       if (!ok) break;
-      ns += (uint32_t)max(0, end - x.a);
-      const int row = t * tp.tpt * p.g + r;  // row of the item
-      if (end <= x.a) {  // this piece holds no key of the tile's rows
-        if (x.slot >= 0 && row_ok) p.part_ml[(long long)x.slot * p.rpi + row] = make_float2(-INFINITY, 0.0f);
-        continue;
+      ns += (uint32_t)count;
+      if (count > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1u, abort_flag, kSitePtcO))) {
+          ok = false;
+          break;
+        }
+        ++no;
+        tc_fence_after();
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&o_full[t], no & 1u, abort_flag, kSitePtcO))) {
-        ok = false;
-        break;
-      }
-      ++no;
-      tc_fence_after();
-      if (x.slot < 0) {
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        const bool none = m_used == -INFINITY;
-        const long long at = (long long)(x.tok0 + tok) * p.Hq + (long long)x.kvh * p.g + head;
-        __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.out) + at * D;
-        const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+      float w_own = 1.0f, w_other = 0.0f;  // dual: weights of A's and B's rows in their sum
+      const float* other = nullptr;
+      if (x.dual) {
+        if (x.b - x.a == 1) {
+          if (t == 1) continue;  // one key tile: A alone
+        } else {
+          const long long row = dual_slot * p.rpi + r;
+          float* po = p.part_o + row * D;
+          const uint32_t use = duals++, qd = warp & 3u;
+          if (t == 1) {
+            ok = warp_wait(&dual_free[qd], (use & 1u) ^ 1u, abort_flag, kSitePtcDual);
+            if (!ok) break;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t u[32];
-          tmem_ld32(tmem + lane_base + o_col + c * 32, u);
-          tmem_wait_ld();
-          if (!row_ok) continue;
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t u[32];
+              tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+              tmem_wait_ld();
+              if (!row_ok) continue;
 #pragma unroll
-          for (int e = 0; e < 32; e += 16) {
-            uint32_t wv[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              wv[i] = none ? 0u
-                           : pack_bf16x2(__uint_as_float(u[e + 2 * i]) * inv, __uint_as_float(u[e + 2 * i + 1]) * inv);
-            if (out32) {
-              stg256(orow + c * 32 + e, wv[0], wv[1], wv[2], wv[3], wv[4], wv[5], wv[6], wv[7]);
-            } else {
-              *reinterpret_cast<uint4*>(orow + c * 32 + e) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
-              *reinterpret_cast<uint4*>(orow + c * 32 + e + 8) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
+              for (int e = 0; e < 32; e += 8)
+                stg256(po + c * 32 + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
             }
+            if (row_ok) p.part_ml[row] = make_float2(m_used, l);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&dual_full[qd]);
+            continue;
+          }
+          ok = warp_wait(&dual_full[qd], use & 1u, abort_flag, kSitePtcDual);
+          if (!ok) break;
+          if (row_ok) {
+            const float2 ml = __ldcg(&p.part_ml[row]);
+            const float mx = fmaxf(m_used, ml.x);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            w_own = ex2_approx(m_used - base);
+            w_other = ex2_approx(ml.x - base);
+            l = l * w_own + ml.y * w_other;
+            m_used = mx;
+            other = po;
           }
         }
-        if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
-      } else {
-        float* po = p.part_o + ((long long)x.slot * p.rpi + row) * D;
+      }
+      // columns [32 c, 32 c + 32) of the row's O, relative to m_used (whole warp)
+      auto load_o = [&](int c, uint32_t (&u)[32]) {
+        tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+        tmem_wait_ld();
+        if (other != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(other + c * 32 + e));
+            u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), w_own, v.x * w_other));
+            u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), w_own, v.y * w_other));
+            u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), w_own, v.z * w_other));
+            u[e + 3] = __float_as_uint(fmaf(__uint_as_float(u[e + 3]), w_own, v.w * w_other));
+          }
+        }
+      };
+      const long long at = (long long)(x.tok0 + tok) * p.Hq + (long long)x.kvh * p.g + head;
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.out) + at * D;
+      const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+      // stores 32 finished columns of the row, u inv
+      auto store_o = [&](int c, const uint32_t (&u)[32], float inv, bool none) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 16) {
+          uint32_t wv[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            wv[i] = none ? 0u
+                         : pack_bf16x2(__uint_as_float(u[e + 2 * i]) * inv, __uint_as_float(u[e + 2 * i + 1]) * inv);
+          if (out32) {
+            stg256(orow + c * 32 + e, wv[0], wv[1], wv[2], wv[3], wv[4], wv[5], wv[6], wv[7]);
+          } else {
+            *reinterpret_cast<uint4*>(orow + c * 32 + e) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+            *reinterpret_cast<uint4*>(orow + c * 32 + e + 8) = make_uint4(wv[4], wv[5], wv[6], wv[7]);
+          }
+        }
+      };
+      if (x.slot < 0) {
+        if (count == 0) continue;  // a tile B without rows
+        const bool none = m_used == -INFINITY;
+        const float inv = none ? 0.0f : 1.0f / l;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t u[32];
-          tmem_ld32(tmem + lane_base + o_col + c * 32, u);
-          tmem_wait_ld();
-          if (!row_ok) continue;
-#pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            stg256(po + c * 32 + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+          load_o(c, u);
+          if (row_ok) store_o(c, u, inv, none);
         }
-        if (row_ok) p.part_ml[(long long)x.slot * p.rpi + row] = make_float2(m_used, l);
+        if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
+      } else if (__any_sync(0xffffffffu, row_ok)) {
+        const int row = (x.dual ? 0 : t * tp.tpt * p.g) + r;  // row of the item
+        const long long own = (long long)x.slot * p.rpi + row;
+        if (count > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t u[32];
+            load_o(c, u);
+            if (!row_ok) continue;
+            float* po = p.part_o + own * D + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              stg256(po + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+          }
+        }
+        // without a key tile here: m = -inf, and its O, not written, is not read
+        if (row_ok) p.part_ml[own] = make_float2(m_used, l);
+        if (x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4)) {
+          const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second
+          const long long pr = x.pieces.slot(1 - mine) * p.rpi + row;
+          const float2 ml = row_ok ? __ldcg(&p.part_ml[pr]) : make_float2(-INFINITY, 0.0f);
+          const float mx = fmaxf(m_used, ml.x);
+          const bool none = mx == -INFINITY, read = row_ok && ml.x != -INFINITY;
+          const float base = none ? 0.0f : mx;
+          const float w_mine = ex2_approx(m_used - base), w_that = ex2_approx(ml.x - base);
+          const float lt = mine ? fmaf(l, w_mine, ml.y * w_that) : fmaf(ml.y, w_that, l * w_mine);
+          const float inv = none ? 0.0f : 1.0f / lt;
+          const float4* src = reinterpret_cast<const float4*>(p.part_o + pr * D);
+          float4 v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t u[32];
+            if (count > 0) {
+              load_o(c, u);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) u[e] = 0u;
+            }
+            const float* f = reinterpret_cast<const float*>(v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {  // first piece, then second: the same sum whichever joins
+              const float a = __uint_as_float(u[e]);
+              u[e] = __float_as_uint(mine ? fmaf(a, w_mine, f[e] * w_that) : fmaf(f[e], w_that, a * w_mine));
+            }
+            if (c + 1 < D / 32) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + 8 * (c + 1) + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            if (row_ok) store_o(c, u, inv, none);
+          }
+          if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (mx + __log2f(lt)) * 0.69314718055994531f;
+        }
+        __syncwarp();
       }
       tc_fence_before();
+      if (x.dual && x.b - x.a > 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dual_free[warp & 3u]);
+      }
     }
   }
 

@@ -14,6 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
+from ._lib import front as _front
 from .errors import InvalidLaunchConfig, check
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
@@ -203,8 +204,10 @@ def attention_bwd_workspace_bytes(B, Hq, S, D, dtype=torch.bfloat16) -> int:
 
 # ---------------------------------------------------------------- position rotation, paged cache
 #
-# These are called once or twice per layer and token: each checks its operands in one expression
-# and looks for the reason only when that fails.
+# These are called once or twice per layer and token, so the usual call goes through beacon_front
+# (csrc/front.cpp: the checks, the outputs and the C call without Python's part of it).  It answers
+# None for operands that it does not take and the status of a call that failed; what follows then checks
+# operand by operand and names the reason.
 
 def _refuse(what, *tests):
     """Raise for the first (holds, message) that does not hold."""
@@ -278,6 +281,10 @@ def qk_norm_rope_fwd(qkv, q_gain, k_gain, table, batch, seq, heads, kv_heads, po
     with gain [D], rotation by the table's row of the token's position (its place in the sequence,
     or positions [B*S] int32), and the layout attention_fwd reads.  A gain of None: no norm for those
     heads; table None: no rotation; rotated width below D: the rest of each head passes through."""
+    r = _front().qk_norm_rope_fwd(qkv, q_gain, k_gain, table, batch, seq, heads, kv_heads, positions, interleaved, eps)
+    if type(r) is tuple:
+        return r
+    check(r or 0)
     n = heads + 2 * kv_heads
     if heads <= 0 or kv_heads <= 0 or qkv.dim() != 2 or qkv.shape[0] != batch * seq or qkv.shape[1] % n:
         raise InvalidLaunchConfig(f"qk_norm_rope_fwd: qkv {tuple(qkv.shape)} is not {batch * seq} rows of "
@@ -297,6 +304,11 @@ def qk_norm_rope_bwd(dq, dk, dv, qkv, q_gain, k_gain, table, positions=None, int
                      workspace=None):
     """(dqkv, dq_gain, dk_gain) of qk_norm_rope_fwd for the gradients of its outputs ([B,H,S,D],
     [B,Hkv,S,D] twice); the norms are formed again from qkv.  A gain of None has no gradient (None)."""
+    if workspace is None:
+        r = _front().qk_norm_rope_bwd(dq, dk, dv, qkv, q_gain, k_gain, table, positions, interleaved, eps)
+        if type(r) is tuple:
+            return r
+        check(r or 0)
     if dq.dim() != 4 or dk.dim() != 4 or dk.shape != dv.shape or qkv.dim() != 2:
         raise InvalidLaunchConfig("qk_norm_rope_bwd: dq [B,H,S,D], dk and dv [B,Hkv,S,D], qkv [B*S, (H + 2 Hkv) D]")
     B, H, S, D = dq.shape
@@ -327,6 +339,12 @@ def qk_norm_rope_append(qkv, q_gain, k_gain, table, k_cache, v_cache, page_table
     pool serve).  Sequence s owns the rows [cu_q[s], cu_q[s+1]) of qkv [T, (H + 2 Hkv) D] and kv_lens[s]
     cached tokens with the new ones last; token j of it sits in page page_table[s][j // page_size].  It
     rotates by j, or by positions [T].  All tables are int32 on the device; nothing is read back."""
+    if q is None:
+        r = _front().qk_norm_rope_append(qkv, q_gain, k_gain, table, k_cache, v_cache, page_table, cu_q, kv_lens, heads,
+                                         positions, interleaved, eps)
+        if isinstance(r, torch.Tensor):
+            return r
+        check(r or 0)
     *paging, Hkv, D, dtype = _paging("qk_norm_rope_append", k_cache, v_cache, page_table, cu_q, kv_lens)
     if qkv.dim() != 2 or qkv.dtype is not dtype:
         raise InvalidLaunchConfig(f"qk_norm_rope_append: qkv {tuple(qkv.shape)} of {qkv.dtype} beside caches of {dtype}")
@@ -354,6 +372,11 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q=0, cau
     keys first.  New token i of a sequence sees the keys up to its own place kv_len - q_len + i (every
     key with causal=False); a token that sees none gets out 0 and lse -inf.  `max_q`, the largest
     number of new tokens of a sequence where the caller knows it, only chooses the kernel."""
+    if out is None and lse is None and workspace is None:
+        r = _front().paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q, causal)
+        if type(r) is tuple:
+            return r
+        check(r or 0)
     seqs, *paging, Hkv, D, dtype = _paging("paged_attention", k_cache, v_cache, page_table, cu_q, kv_lens)
     code = _DT.get(dtype)
     if q.dim() != 3 or q.shape[2] != D or q.dtype is not dtype or not q.is_cuda or code is None:
