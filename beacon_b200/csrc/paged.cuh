@@ -34,7 +34,7 @@ struct PagedParams {
   float* lse;                // [tokens, Hq] or null
   int sched_slot;            // row of g_paged_done
   int4* heads;               // [gridDim.x] the split item that begins in this CTA's run (paged_head)
-  float* part_o;             // [2 * gridDim.x, rpi, D]
+  float* part_o;             // [slots, D / 4, rpi, 4] (paged_part)
   float2* part_ml;           // [2 * gridDim.x, rpi] (running maximum, in log2 units; sum)
 };
 
@@ -192,6 +192,13 @@ __device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem
 }
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
 __device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
+
+// Columns [4 c, 4 c + 4) of row r of a workspace slot.  Rows lie side by side: the kernels hold a row per
+// thread, and 32 of them store or load 512 contiguous bytes (a row-major slot made the end of a split
+// piece cost 14 us, mostly in its uncoalesced accesses).
+__device__ __forceinline__ float4* paged_part(const PagedParams& p, long long slot, int c, int r) {
+  return reinterpret_cast<float4*>(p.part_o) + (slot * (p.D / 4) + c) * p.rpi + r;
+}
 
 // The runs that hold pieces of a split item: a run's first piece may continue an item, its last may begin one.
 struct PagedPieces {
@@ -399,82 +406,90 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
         for (int c = 0; c < CT; ++c) stf((T*)p.out + at * D + tx + 16 * c, o[i][c] * inv);
         if (tx == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
       } else {
-        float* po = p.part_o + ((long long)slot * p.rpi + r) * D;
+        float* po = reinterpret_cast<float*>(paged_part(p, slot, tx / 4, r)) + tx % 4;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) po[tx + 16 * c] = o[i][c];
+        for (int c = 0; c < CT; ++c) po[(long long)(4 * c) * p.rpi * 4] = o[i][c];  // column tx + 16 c
         if (tx == 0) p.part_ml[(long long)slot * p.rpi + r] = make_float2(m * 1.4426950408889634f, l);
       }
     }
   }
 }
 
-// Joins the split items that p.heads lists: all their rows are dealt out to the grid's warps.  The item that
-// begins in run c has its first piece in slot 2c + 1 and the others in slots 2(c + 1), 2(c + 2), .. in
-// order.  With M = max m: out = sum 2^(m - M) O / sum 2^(m - M) l.
+// Joins the split items that p.heads lists: their blocks of 32 rows x 16 columns are dealt out to the
+// grid's warps, a row per lane.  The item that begins in run c has its first piece in slot 2c + 1 and
+// the others in slots 2(c + 1), 2(c + 2), .. in order.  With M = max m:
+// out = sum 2^(m - M) O / sum 2^(m - M) l.
 constexpr int kPagedMostRuns = 320;  // of any attention kernel that leaves its joins to this one
 template <typename T>
-__global__ void __launch_bounds__(512) k_paged_join(const PagedParams p, int runs) {
+__global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int runs) {
   __shared__ int4 heads[kPagedMostRuns];
-  __shared__ int first[kPagedMostRuns + 1];  // rows of the items before
+  __shared__ int first[kPagedMostRuns + 1];  // 32-row blocks of the items before
   pdl_wait();
   const int lane = (int)lane_id();
-  for (int c = (int)threadIdx.x; c < runs; c += 512) heads[c] = p.heads[c];
+  for (int c = (int)threadIdx.x; c < runs; c += 256) heads[c] = p.heads[c];
   __syncthreads();
   if (warp_id() == 0) {
     int sum = 0;
     for (int c0 = 0; c0 < runs; c0 += 32) {
-      const int rows = c0 + lane < runs ? heads[c0 + lane].w & 0xffff : 0;
-      int end = rows;
+      const int blocks = c0 + lane < runs ? ((heads[c0 + lane].w & 0xffff) + 31) / 32 : 0;
+      int end = blocks;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, end, o);
         if (lane >= o) end += v;
       }
-      if (c0 + lane < runs) first[c0 + lane] = sum + end - rows;
+      if (c0 + lane < runs) first[c0 + lane] = sum + end - blocks;
       sum += __shfl_sync(0xffffffffu, end, 31);
     }
     if (lane == 0) first[runs] = sum;
   }
   __syncthreads();
-  const int total = first[runs];
-  constexpr int CPL = 4;  // columns per lane
-  const bool on = CPL * lane < p.D;
-  for (int k = (int)(blockIdx.x * 16 + warp_id()); k < total; k += (int)gridDim.x * 16) {
+  const int parts = p.D / 16, total = first[runs] * parts;
+  for (int k = (int)(blockIdx.x * 8 + warp_id()); k < total; k += (int)gridDim.x * 8) {
+    const int block = k / parts, c0 = (k - block * parts) * 4;
     int c = 0;
     for (int step = 256; step > 0; step >>= 1)
-      if (c + step < runs && first[c + step] <= k) c += step;  // the last item that starts at or before row k
+      if (c + step < runs && first[c + step] <= block) c += step;  // the last item that starts at or before it
     const int4 h = heads[c];
-    const int r = k - first[c], pieces = h.w >> 16;
-    const PagedPieces pc{c, pieces};
+    const int r = (block - first[c]) * 32 + lane, rows = h.w & 0xffff;
+    const PagedPieces pc{c, h.w >> 16};
+    if (r >= rows) continue;
     float mx = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) mx = fmaxf(mx, p.part_ml[pc.slot(i) * p.rpi + r].x);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+#pragma unroll 8
+    for (int i = 0; i < pc.n; ++i) mx = fmaxf(mx, p.part_ml[pc.slot(i) * p.rpi + r].x);
     const float base = mx == -INFINITY ? 0.0f : mx;
-    float l = 0.0f, o[CPL] = {};
+    float l = 0.0f, o[16] = {};
 #pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-      const long long at = pc.slot(i) * p.rpi + r;
-      const float2 ml = p.part_ml[at];
-      const bool have = on && ml.x != -INFINITY;  // a piece without a key of this row has no O
-      const float4 v = have ? *reinterpret_cast<const float4*>(p.part_o + at * p.D + CPL * lane)
-                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const float wgt = exp2f(ml.x - base);
+    for (int i = 0; i < pc.n; ++i) {
+      const float2 ml = p.part_ml[pc.slot(i) * p.rpi + r];
+      // a piece without a key of this row has left old values in its slot: read all the same, so that no
+      // load waits for another, and passed over
+      const bool have = ml.x != -INFINITY;
+      const float wgt = have ? exp2f(ml.x - base) : 0.0f;
       l = fmaf(ml.y, wgt, l);
-      o[0] = fmaf(v.x, wgt, o[0]);
-      o[1] = fmaf(v.y, wgt, o[1]);
-      o[2] = fmaf(v.z, wgt, o[2]);
-      o[3] = fmaf(v.w, wgt, o[3]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = *paged_part(p, pc.slot(i), c0 + q, r);
+        o[4 * q] = have ? fmaf(v.x, wgt, o[4 * q]) : o[4 * q];
+        o[4 * q + 1] = have ? fmaf(v.y, wgt, o[4 * q + 1]) : o[4 * q + 1];
+        o[4 * q + 2] = have ? fmaf(v.z, wgt, o[4 * q + 2]) : o[4 * q + 2];
+        o[4 * q + 3] = have ? fmaf(v.w, wgt, o[4 * q + 3]) : o[4 * q + 3];
+      }
     }
     const int fr = h.z + r;
     const long long at = (long long)(h.x + fr / p.g) * p.Hq + (long long)h.y * p.g + fr % p.g;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (on) {
+    T* dst = (T*)p.out + at * p.D + 4 * c0;
 #pragma unroll
-      for (int e = 0; e < CPL; ++e) stf((T*)p.out + at * p.D + CPL * lane + e, o[e] * inv);
+    for (int e = 0; e < 16; ++e) o[e] *= inv;
+    if ((reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+      store8(dst, *reinterpret_cast<const float(*)[8]>(&o[0]));
+      store8(dst + 8, *reinterpret_cast<const float(*)[8]>(&o[8]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) stf(dst + e, o[e]);
     }
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[at] = l > 0.0f ? (base + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    if (c0 == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? (base + log2f(l)) * 0.69314718055994531f : -INFINITY;
   }
 }
 

@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
     fence_mbarrier_init();
   }
   __syncthreads();
+  pdl_wait();
 
   // fragment addresses within a tile: chunk c of key r lies at chunk c ^ (r & 7) of its row
   const int kr = (lane & 7) + ((lane >> 4) << 3), kcb = (lane >> 3) & 1;  // K: keys x head dims
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
         store_row(x, r, mx, lt, ot);
         continue;
       }
-      float* po = p.part_o + (slot * p.rpi + r) * D + CPL * lane;
+      float* po = p.part_o + (slot * p.rpi + r) * D + CPL * lane;  // row-major slots: a warp holds one row
 #pragma unroll
       for (int e = 0; e < CPL; ++e) po[e] = ot[e];
       if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);

@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();  // everything above runs while the kernel before this one ends
 
   auto read_item = [&](int ci, PtcItem& x) -> bool {
     const int s = ci % kPtcItems;
@@ -544,14 +545,21 @@ __global__ void __launch_bounds__(384, 1)
         ++no;
         tc_fence_after();
       }
+      // 32 columns of the row into a workspace slot
+      auto store_part = [&](float4* dst, const uint32_t (&u)[32]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          dst[(long long)e * p.rpi] = make_float4(__uint_as_float(u[4 * e]), __uint_as_float(u[4 * e + 1]),
+                                                  __uint_as_float(u[4 * e + 2]), __uint_as_float(u[4 * e + 3]));
+      };
       float w_own = 1.0f, w_other = 0.0f;  // dual: weights of A's and B's rows in their sum
-      const float* other = nullptr;
+      const float4* other = nullptr;
       if (x.dual) {
         if (x.b - x.a == 1) {
           if (t == 1) continue;  // one key tile: A alone
         } else {
           const long long row = dual_slot * p.rpi + r;
-          float* po = p.part_o + row * D;
+          float4* po = paged_part(p, dual_slot, 0, r);
           const uint32_t use = duals++, qd = warp & 3u;
           if (t == 1) {
             ok = warp_wait(&dual_free[qd], (use & 1u) ^ 1u, abort_flag, kSitePtcDual);
@@ -561,10 +569,7 @@ __global__ void __launch_bounds__(384, 1)
               uint32_t u[32];
               tmem_ld32(tmem + lane_base + o_col + c * 32, u);
               tmem_wait_ld();
-              if (!row_ok) continue;
-#pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                stg256(po + c * 32 + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+              if (row_ok) store_part(po + (long long)(8 * c) * p.rpi, u);
             }
             if (row_ok) p.part_ml[row] = make_float2(m_used, l);
             tc_fence_before();
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(384, 1)
         if (other != nullptr) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(other + c * 32 + e));
+            const float4 v = __ldcg(other + (long long)(8 * c + e / 4) * p.rpi);
             u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), w_own, v.x * w_other));
             u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), w_own, v.y * w_other));
             u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), w_own, v.z * w_other));
@@ -640,29 +645,25 @@ __global__ void __launch_bounds__(384, 1)
           for (int c = 0; c < D / 32; ++c) {
             uint32_t u[32];
             load_o(c, u);
-            if (!row_ok) continue;
-            float* po = p.part_o + own * D + c * 32;
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              stg256(po + e, u[e], u[e + 1], u[e + 2], u[e + 3], u[e + 4], u[e + 5], u[e + 6], u[e + 7]);
+            if (row_ok) store_part(paged_part(p, x.slot, 8 * c, row), u);
           }
         }
         // without a key tile here: m = -inf, and its O, not written, is not read
         if (row_ok) p.part_ml[own] = make_float2(m_used, l);
         if (x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4)) {
           const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second
-          const long long pr = x.pieces.slot(1 - mine) * p.rpi + row;
-          const float2 ml = row_ok ? __ldcg(&p.part_ml[pr]) : make_float2(-INFINITY, 0.0f);
+          const long long that = x.pieces.slot(1 - mine);
+          const float2 ml = row_ok ? __ldcg(&p.part_ml[that * p.rpi + row]) : make_float2(-INFINITY, 0.0f);
           const float mx = fmaxf(m_used, ml.x);
           const bool none = mx == -INFINITY, read = row_ok && ml.x != -INFINITY;
           const float base = none ? 0.0f : mx;
           const float w_mine = ex2_approx(m_used - base), w_that = ex2_approx(ml.x - base);
           const float lt = mine ? fmaf(l, w_mine, ml.y * w_that) : fmaf(ml.y, w_that, l * w_mine);
           const float inv = none ? 0.0f : 1.0f / lt;
-          const float4* src = reinterpret_cast<const float4*>(p.part_o + pr * D);
+          const float4* src = paged_part(p, that, 0, row);
           float4 v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)e * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t u[32];
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (c + 1 < D / 32) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + 8 * (c + 1) + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)(8 * (c + 1) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             if (row_ok) store_o(c, u, inv, none);
           }
