@@ -47,6 +47,7 @@ EXPORTS = (
     "beacon_rope_table", "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd",
     "beacon_qk_norm_rope_bwd_workspace_size", "beacon_qk_norm_rope_append",
     "beacon_paged_attention_fwd", "beacon_paged_attention_workspace_size",
+    "beacon_llama_block_paged_fwd", "beacon_llama_block_paged_workspace_size",
     "beacon_residual_add_fwd", "beacon_residual_add_bwd", "beacon_cast",
     "beacon_embedding_lookup_fwd", "beacon_embedding_lookup_bwd", "beacon_dropout_fwd", "beacon_dropout_bwd",
     "beacon_arena_create", "beacon_arena_destroy", "beacon_arena_base", "beacon_arena_size", "beacon_launch",
@@ -148,6 +149,9 @@ def lib():
     _sig(L, "beacon_paged_attention_fwd", _int,
          [_vp] * 3 + [_i64] + [_vp] * 5 + [_i64] * 13 + [_int, _int, _vp, _sz, _vp])
     _sig(L, "beacon_paged_attention_workspace_size", _sz, [_i64, _int])
+    _sig(L, "beacon_llama_block_paged_fwd", _int,
+         [_vp] * 12 + [_i64] * 2 + [_int] + [_vp] * 5 + [_i64] * 15 + [ctypes.c_float, _int, _vp, _sz, _vp])
+    _sig(L, "beacon_llama_block_paged_workspace_size", _sz, [_i64] * 6 + [_int])
     _sig(L, "beacon_residual_add_fwd", _int, [_vp, _vp, _vp, _i64, _int, _vp])
     _sig(L, "beacon_residual_add_bwd", _int, [_vp, _vp, _vp, _i64, _int, _vp])
     _sig(L, "beacon_cast", _int, [_vp, _vp, _i64, _int, _vp])

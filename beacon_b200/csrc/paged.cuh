@@ -252,31 +252,41 @@ __device__ __forceinline__ long long paged_key(const PagedSeqs& g, int seq, int 
 }
 
 // ---------------------------------------------------------------------------
-// Exact path: float32 (and bf16 caches whose pages TMA cannot describe), fp32 FFMA, expf.
-// 256 threads; tiles of BM rows x 64 keys; Q, K, V and P in shared memory as fp32, each thread
-// BM/16 rows x 4 keys of S and BM/16 rows x D/16 columns of O in registers.
+// Exact path: float32 (and bf16 calls that the other kernels' loads cannot serve), fp32 FFMA, expf.
+//
+// 256 threads; items of 64 rows, tiles of 64 keys; Q, K, V and P in shared memory as fp32.  Thread
+// (ty, tx) of 16 x 16 holds rows ty + 16 i: 4 keys of S each and D/16 columns of O; a warp without a row
+// of the item skips the arithmetic, so a decode step pays for its few rows only.  K and V of the next
+// tile are copied while this one is used (cp.async where rows are 16-byte aligned), its cache offsets
+// looked up one tile earlier still.  Bound: FFMA and shared-memory loads for full items (two 16-byte
+// loads per 16 FMA), HBM latency for short ones.
 // ---------------------------------------------------------------------------
-constexpr int kPagedSimtKt = 64;
-template <int D, int BM>
+constexpr int kPagedSimtKt = 64, kPagedSimtRows = 64;
+template <int D>
 constexpr size_t paged_simt_smem() {
-  return sizeof(float) * ((size_t)(BM + 2 * kPagedSimtKt) * (D + 4) + (size_t)BM * (kPagedSimtKt + 4) + 2 * BM);
+  return sizeof(float) * ((size_t)(kPagedSimtRows + 4 * kPagedSimtKt) * (D + 4) +
+                          (size_t)kPagedSimtRows * (kPagedSimtKt + 4) + 2 * kPagedSimtRows) +
+         sizeof(long long) * 2 * kPagedSimtKt;
 }
 
-template <typename T, int D, int BM>
+// ASYNC: T is float and the caches' rows are 16-byte aligned.
+template <typename T, int D, bool ASYNC>
 __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q, const T* __restrict__ kc,
                                                          const T* __restrict__ vc, const PagedParams p) {
-  constexpr int KT = kPagedSimtKt, LD = D + 4, LP = KT + 4, RT = BM / 16, CT = D / 16;
+  constexpr int KT = kPagedSimtKt, BM = kPagedSimtRows, LD = D + 4, LP = KT + 4, RT = BM / 16, CT = D / 16;
+  constexpr int CV = CT < 4 ? CT : 4;  // columns per load: tx * CV + 16 CV g + e
   extern __shared__ __align__(16) float fsm[];
   float* sq = fsm;
-  float* sk = sq + BM * LD;
-  float* sv = sk + KT * LD;
-  float* sp = sv + KT * LD;
+  float* sk = sq + BM * LD;             // [2][KT]
+  float* sv = sk + 2 * KT * LD;         // [2][KT]
+  float* sp = sv + 2 * KT * LD;
   float* s_m = sp + BM * LP;
   float* s_l = s_m + BM;
+  long long* s_off = reinterpret_cast<long long*>(s_l + BM);  // [2][KT] cache offsets of a tile's keys, -1: none
   __shared__ PagedItem item;
   __shared__ int more;
   const int tid = (int)threadIdx.x;
-  const int ty = tid >> 4, tx = tid & 15;  // S rows ty + 16 i, keys tx + 16 j; O columns tx + 16 c
+  const int ty = tid >> 4, tx = tid & 15;
   pdl_launch_dependents();
   PagedWalk walk;
   if (warp_id() == 0) {
@@ -299,7 +309,41 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
     if (!more) break;
     const PagedItem x = item;
     const int rows = min(p.rpi, x.q_len * group - x.row0);
-    for (int e = tid; e < BM * D; e += 256) {
+    const bool works = (ty & ~1) < rows;  // the warp has a row
+    auto lookup = [&](int j, int buf) {
+      if (tid < KT) {
+        const int key = j * KT + tid;
+        s_off[buf * KT + tid] = j < x.b && key < x.kv ? paged_key(p.pg, x.seq, x.kvh, key) : -1;
+      }
+    };
+    auto copy = [&](int buf) {
+      for (int e = tid; e < KT * (D / 4); e += 256) {
+        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+        const long long at = s_off[buf * KT + r];
+        float* dk = sk + (buf * KT + r) * LD + d;
+        float* dv = sv + (buf * KT + r) * LD + d;
+        if constexpr (ASYNC) {
+          const bool have = at >= 0;
+          cp_async16_or_zero(smem_u32(dk), kc + (have ? at + d : 0), have);
+          cp_async16_or_zero(smem_u32(dv), vc + (have ? at + d : 0), have);
+        } else {
+          float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
+          if (at >= 0) {
+            const T *ks = kc + at + d, *vs = vc + at + d;
+            kf = make_float4(ldf(ks), ldf(ks + 1), ldf(ks + 2), ldf(ks + 3));
+            vf = make_float4(ldf(vs), ldf(vs + 1), ldf(vs + 2), ldf(vs + 3));
+          }
+          *reinterpret_cast<float4*>(dk) = kf;
+          *reinterpret_cast<float4*>(dv) = vf;
+        }
+      }
+      cp_async_commit();
+    };
+    lookup(x.a, 0);
+    __syncthreads();
+    copy(0);
+    lookup(x.a + 1, 1);
+    for (int e = tid; e < min(BM, (rows + 15) & ~15) * D; e += 256) {
       const int r = e / D, d = e % D;
       float v = 0.0f;
       if (r < rows) {
@@ -314,30 +358,28 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
     }
     float o[RT][CT] = {};
     for (int j = x.a; j < x.b; ++j) {
-      const int k0 = j * KT;
-      __syncthreads();
-      for (int e = tid; e < KT * (D / 4); e += 256) {
-        const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-        float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
-        if (k0 + r < x.kv) {
-          const long long at = paged_key(p.pg, x.seq, x.kvh, k0 + r);
-          if (at >= 0) {
-            kf = make_float4(ldf(kc + at + d), ldf(kc + at + d + 1), ldf(kc + at + d + 2), ldf(kc + at + d + 3));
-            vf = make_float4(ldf(vc + at + d), ldf(vc + at + d + 1), ldf(vc + at + d + 2), ldf(vc + at + d + 3));
-          }
-        }
-        *reinterpret_cast<float4*>(sk + r * LD + d) = kf;
-        *reinterpret_cast<float4*>(sv + r * LD + d) = vf;
+      const int k0 = j * KT, buf = (j - x.a) & 1;
+      __syncthreads();  // the next tile's offsets are there, and its buffer has been used
+      if (j + 1 < x.b) {
+        copy(buf ^ 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
       }
       __syncthreads();
+      if (j + 2 < x.b) lookup(j + 2, buf);
+      if (!works) continue;
+      const float* kt = sk + buf * KT * LD;
+      const float* vt = sv + buf * KT * LD;
       float s[RT][4] = {};
 #pragma unroll 4
       for (int d = 0; d < D; d += 4) {
         float4 kf[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * LD + d);
+        for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(kt + (tx + 16 * c) * LD + d);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
+          if (i > 0 && 16 * i >= rows) break;
           const float4 qf = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * LD + d);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -346,6 +388,7 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
       }
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
+        if (i > 0 && 16 * i >= rows) break;
         const int r = ty + 16 * i;
         const int limit = (r < rows ? paged_limit(p, x, x.row0 + r) : 0) - k0;
         float mx = -INFINITY;
@@ -376,21 +419,30 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
 #pragma unroll
         for (int c = 0; c < CT; ++c) o[i][c] *= alpha;
       }
-      __syncthreads();
+      __syncwarp();  // a row's probabilities are written and read by one warp
 #pragma unroll 4
-      for (int kk = 0; kk < KT; ++kk) {
-        float vf[CT];
+      for (int kk = 0; kk < KT; kk += 4) {
+        float vf[4][CT];
 #pragma unroll
-        for (int c = 0; c < CT; ++c) vf[c] = sv[kk * LD + tx + 16 * c];
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int c = 0; c < CT; c += CV) {
+            const float* src = vt + (kk + e) * LD + tx * CV + 16 * c;
+            if constexpr (CV == 4) *reinterpret_cast<float4*>(&vf[e][c]) = *reinterpret_cast<const float4*>(src);
+            else if constexpr (CV == 2) *reinterpret_cast<float2*>(&vf[e][c]) = *reinterpret_cast<const float2*>(src);
+            else vf[e][c] = *src;
+          }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-          const float pf = sp[(ty + 16 * i) * LP + kk];
+          if (i > 0 && 16 * i >= rows) break;
+          const float4 pf = *reinterpret_cast<const float4*>(sp + (ty + 16 * i) * LP + kk);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) o[i][c] = fmaf(pf, vf[c], o[i][c]);
+          for (int c = 0; c < CT; ++c)
+            o[i][c] = fmaf(pf.w, vf[3][c], fmaf(pf.z, vf[2][c], fmaf(pf.y, vf[1][c], fmaf(pf.x, vf[0][c], o[i][c]))));
         }
       }
     }
-    __syncthreads();
+    __syncwarp();
     const bool whole = x.a == 0 && x.b == x.n;
     const int slot = paged_slot(x);
 #pragma unroll
@@ -398,19 +450,18 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
       const int r = ty + 16 * i;
       if (r >= rows) continue;
       const float m = s_m[r], l = s_l[r];
-      if (whole) {
-        const int fr = x.row0 + r;
-        const long long at = (long long)(x.q0 + fr / group) * p.Hq + (long long)x.kvh * group + fr % group;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const int fr = x.row0 + r;
+      const long long at = (long long)(x.q0 + fr / group) * p.Hq + (long long)x.kvh * group + fr % group;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-        for (int c = 0; c < CT; ++c) stf((T*)p.out + at * D + tx + 16 * c, o[i][c] * inv);
-        if (tx == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
-      } else {
-        float* po = reinterpret_cast<float*>(paged_part(p, slot, tx / 4, r)) + tx % 4;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) po[(long long)(4 * c) * p.rpi * 4] = o[i][c];  // column tx + 16 c
-        if (tx == 0) p.part_ml[(long long)slot * p.rpi + r] = make_float2(m * 1.4426950408889634f, l);
+      for (int c = 0; c < CT; ++c) {
+        const int d = tx * CV + 16 * (c - c % CV) + c % CV;
+        if (whole) stf((T*)p.out + at * D + d, o[i][c] * inv);
+        else reinterpret_cast<float*>(paged_part(p, slot, d / 4, r))[d % 4] = o[i][c];
       }
+      if (tx != 0) continue;
+      if (!whole) p.part_ml[(long long)slot * p.rpi + r] = make_float2(m * 1.4426950408889634f, l);
+      else if (p.lse != nullptr) p.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
     }
   }
 }

@@ -551,6 +551,43 @@ def llama_block_fwd_folded(x, w_qkv_folded, w_o, w_gate_folded, w_up_folded, w_d
     return out
 
 
+def llama_block_paged_workspace_bytes(tokens, d_model, heads, kv_heads, head_dim, d_ff) -> int:
+    return int(_lib.lib().beacon_llama_block_paged_workspace_size(tokens, d_model, heads, kv_heads, head_dim, d_ff,
+                                                                  _lib.BF16))
+
+
+def llama_block_paged_fwd(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_down, k_cache, v_cache, page_table, cu_q,
+                          kv_lens, heads, table=None, q_gain=None, k_gain=None, max_q=0, interleaved=False, eps=1e-5,
+                          out=None, workspace=None):
+    """llama_block_fwd for the new tokens x [T, d_model] of a batch of sequences with cached keys and values
+    (tables as in qk_norm_rope_append): h = x + attn(rope(norm(rmsnorm(x) Wqkv)), cache) Wo;
+    out = h + swiglu(rmsnorm(h)).  The new tokens' keys and values are written to the pages."""
+    seqs, *paging, Hkv, D, dtype = _paging("llama_block_paged_fwd", k_cache, v_cache, page_table, cu_q, kv_lens)
+    T, dm = x.shape
+    dt = _dtype(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_down, q_gain, k_gain)
+    if x.dtype is not dtype:
+        raise InvalidLaunchConfig(f"llama_block_paged_fwd: x of {x.dtype} beside caches of {dtype}")
+    if w_qkv.shape != (dm, (heads + 2 * Hkv) * D) or w_o.shape != (heads * D, dm):
+        raise InvalidLaunchConfig(f"llama_block_paged_fwd: w_qkv {tuple(w_qkv.shape)} and w_o {tuple(w_o.shape)} do not "
+                                  f"fit {heads} + 2 x {Hkv} heads of {D}")
+    for g in (q_gain, k_gain):
+        if g is not None and g.numel() != D:
+            raise InvalidLaunchConfig(f"llama_block_paged_fwd: gains must have {D} elements")
+    if table is not None and not (table.dtype is torch.float32 and table.dim() == 2 and table.is_cuda
+                                  and table.is_contiguous()):
+        raise InvalidLaunchConfig("llama_block_paged_fwd: the rotation table must be a contiguous float32 CUDA matrix")
+    rows, rot = (0, 0) if table is None else table.shape
+    if out is None:
+        out = torch.empty_like(x)
+    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    check(_lib.lib().beacon_llama_block_paged_fwd(
+        _p(out), _p(x), _p(attn_norm), _p(w_qkv), _p(q_gain), _p(k_gain), _p(w_o), _p(ffn_norm), _p(w_gate), _p(w_up),
+        _p(w_down), _p(table), rows, rot, int(interleaved), _p(k_cache), _p(v_cache), _p(cu_q), _p(kv_lens),
+        _p(page_table), T, seqs, int(max_q or 0), *paging, dm, heads, Hkv, D, w_gate.shape[1], eps, dt, ws, wsb,
+        _stream()))
+    return out
+
+
 # ---------------------------------------------------------------- elementwise
 
 def residual_add(a, b):

@@ -409,6 +409,27 @@ int beacon_paged_attention_fwd(void* out, float* lse, const void* q, int64_t q_s
                                size_t workspace_bytes, void* stream);
 size_t beacon_paged_attention_workspace_size(int64_t head_dim, int dtype);
 
+/* beacon_llama_block_fwd on new tokens of sequences with cached keys and values: x, out [tokens, d_model],
+ * the tokens of all sequences one after another as cu_q says, prompt chunks and single tokens mixed as they
+ * come.  Per-head norms (q_gain, k_gain [head_dim], NULL: none) and the rotation (rope_table NULL with
+ * rot_dim 0: none) act on queries and keys before the new keys and values enter the pages; attention is
+ * causal over the whole cache.  bf16; the other conditions are beacon_llama_block_fwd's and
+ * beacon_paged_attention_fwd's.  Scratch: beacon_llama_block_paged_workspace_size bytes or the library's.
+ * Nothing is read back, so a step can be captured.  Rows of out for tokens that no sequence owns are
+ * undefined. */
+int beacon_llama_block_paged_fwd(void* out, const void* x, const void* attn_norm, const void* w_qkv,
+                                 const void* q_gain, const void* k_gain, const void* w_o, const void* ffn_norm,
+                                 const void* w_gate, const void* w_up, const void* w_down, const float* rope_table,
+                                 int64_t table_positions, int64_t rot_dim, int interleaved, void* k_cache,
+                                 void* v_cache, const int32_t* cu_q, const int32_t* kv_lens,
+                                 const int32_t* page_table, int64_t tokens, int64_t seqs, int64_t max_q,
+                                 int64_t max_pages, int64_t table_stride, int64_t num_pages, int64_t page_size,
+                                 int64_t page_stride, int64_t head_stride, int64_t token_stride, int64_t d_model,
+                                 int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t d_ff, float eps,
+                                 int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t beacon_llama_block_paged_workspace_size(int64_t tokens, int64_t d_model, int64_t heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t d_ff, int dtype);
+
 /* ---- elementwise: crates/beacon-cuda/src/elementwise.rs -------------------- */
 
 /* residual_add (elementwise.rs:47-55): out = a + b */

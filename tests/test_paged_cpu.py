@@ -19,7 +19,10 @@ APPEND = dict(q=H, kc=H, vc=H, qkv=H, ld=512, qg=H, kg=H, table=H, rows=16, pos=
               seqs=2, **PAGES, heads=4, kv=2, D=64, rot=64, inter=0, eps=1e-5, dtype=_lib.BF16, stream=None)
 ATTN = dict(out=H, lse=H, q=H, qs=256, kc=H, vc=H, cu=H, kv_lens=H, pt=H, tokens=3, seqs=2, max_q=0, **PAGES, heads=4,
             kv=2, D=64, causal=1, dtype=_lib.BF16, ws=None, wsb=0, stream=None)
-ENTRY = dict(fwd=("beacon_qk_norm_rope_fwd", FWD), bwd=("beacon_qk_norm_rope_bwd", BWD),
+BLOCK = dict(out=H, x=H, attn_norm=H, w_qkv=H, qg=H, kg=H, w_o=H, ffn_norm=H, w_gate=H, w_up=H, w_down=H, table=H,
+             rows=16, rot=64, inter=0, kc=H, vc=H, cu=H, kv_lens=H, pt=H, tokens=3, seqs=2, max_q=0, **PAGES, dm=128,
+             heads=4, kv=2, D=64, F=256, eps=1e-5, dtype=_lib.BF16, ws=None, wsb=0, stream=None)
+ENTRY = dict(block=("beacon_llama_block_paged_fwd", BLOCK), fwd=("beacon_qk_norm_rope_fwd", FWD), bwd=("beacon_qk_norm_rope_bwd", BWD),
              append=("beacon_qk_norm_rope_append", APPEND), attn=("beacon_paged_attention_fwd", ATTN))
 
 INV, SHAPE, UNIMPL = _lib.ERR_INVALID_LAUNCH_CONFIG, _lib.ERR_SHAPE_MISMATCH, _lib.ERR_UNIMPLEMENTED
@@ -33,7 +36,9 @@ def call(which, **change):
 
 NULLS = dict(fwd=("q", "k", "qkv", "table"), bwd=("dqkv", "dq", "dk", "qkv", "table"),
              append=("q", "kc", "vc", "qkv", "table", "cu", "kv_lens", "pt"),
-             attn=("out", "q", "kc", "vc", "cu", "kv_lens", "pt"))
+             attn=("out", "q", "kc", "vc", "cu", "kv_lens", "pt"),
+             block=("out", "x", "attn_norm", "w_qkv", "w_o", "ffn_norm", "w_gate", "w_up", "w_down", "table", "kc", "vc",
+                    "cu", "kv_lens", "pt"))
 
 
 @pytest.mark.parametrize("which,arg", [(w, a) for w, args in NULLS.items() for a in args])
@@ -57,6 +62,9 @@ def test_null_pointers(which, arg):
     ("attn", dict(qs=255), SHAPE), ("attn", dict(seqs=-1), INV), ("attn", dict(tokens=-1), INV),
     ("attn", dict(max_q=-1), INV), ("attn", dict(page=-16), INV), ("attn", dict(page_stride=-5), SHAPE),
     ("attn", dict(kv=0), INV), ("attn", dict(tokens=1 << 31), INV),
+    ("block", dict(dtype=_lib.F32), UNIMPL), ("block", dict(D=32, rot=32), UNIMPL), ("block", dict(heads=5), SHAPE),
+    ("block", dict(dm=100), INV), ("block", dict(x=H + 2), INV), ("block", dict(page=0), INV),
+    ("block", dict(table_stride=1), SHAPE), ("block", dict(rot=33), SHAPE), ("block", dict(tokens=-1), INV),
 ])
 def test_refusals(which, change, status):
     assert call(which, **change) == status, _lib.last_error()
@@ -65,7 +73,7 @@ def test_refusals(which, change, status):
 
 def test_nothing_to_do_needs_no_device():
     for which, change in (("fwd", dict(batch=0)), ("fwd", dict(seq=0)), ("append", dict(tokens=0)),
-                          ("append", dict(seqs=0)), ("attn", dict(tokens=0)), ("attn", dict(seqs=0))):
+                          ("append", dict(seqs=0)), ("block", dict(tokens=0)), ("attn", dict(tokens=0)), ("attn", dict(seqs=0))):
         assert call(which, **change) == _lib.OK, _lib.last_error()
 
 
@@ -77,6 +85,8 @@ def test_table_and_workspace_sizes():
     assert L.beacon_rope_table(None, 0, 64, 1e4, None) == _lib.OK
     assert L.beacon_paged_attention_workspace_size(128, _lib.BF16) > 0
     assert L.beacon_paged_attention_workspace_size(0, _lib.BF16) == 0
+    assert L.beacon_llama_block_paged_workspace_size(64, 4096, 32, 8, 128, 14336, _lib.BF16) > 64 * 14336 * 2
+    assert L.beacon_llama_block_paged_workspace_size(64, 4096, 32, 8, 96, 14336, _lib.BF16) == 0
     assert L.beacon_qk_norm_rope_bwd_workspace_size(128) >= 148 * 2 * 128 * 4
     assert L.beacon_qk_norm_rope_bwd_workspace_size(0) == 0
 

@@ -314,6 +314,60 @@ def test_prompt_in_chunks_equals_the_training_forward():
     assert np.abs(to_np(lse) - lse64).max() <= LSE_TOL
 
 
+def test_block_over_chunks_and_single_tokens():
+    """The pre-norm block on two sequences' prompts in ragged chunks, then on single tokens, against the
+    whole sequences in 64 bits (the framework's bf16 tolerance)."""
+    import torch
+    from beacon_b200 import ops
+    from helpers import BF16_TOL
+    dm, H, K, D, F, page, lens = 256, 4, 2, 64, 384, 16, (75, 40)
+    r = as_bf16
+    w = dict(attn_norm=r(1 + 0.1 * normal((dm,), 1)), w_qkv=r(normal((dm, (H + 2 * K) * D), 2, std=0.05)),
+             w_o=r(normal((H * D, dm), 3, std=0.05)), ffn_norm=r(1 + 0.1 * normal((dm,), 4)),
+             w_gate=r(normal((dm, F), 5, std=0.05)), w_up=r(normal((dm, F), 6, std=0.05)),
+             w_down=r(normal((F, dm), 7, std=0.05)))
+    gq, gk = r(1 + 0.2 * normal((D,), 8)), r(1 + 0.2 * normal((D,), 9))
+    xs = [r(normal((n, dm), 10 + i)) for i, n in enumerate(lens)]
+    t64 = R.table64(max(lens), D).astype(np.float32).astype(np.float64)
+
+    def rms(a, g):
+        return a / np.sqrt((a * a).mean(-1, keepdims=True) + 1e-5) * g
+
+    refs = []
+    for x in xs:
+        n, x = len(x), x.astype(np.float64)
+        qkv = (rms(x, w["attn_norm"]) @ w["w_qkv"]).reshape(n, H + 2 * K, D)
+        q, k = (R.norm_rope(a, g, t64, np.arange(n), False) for a, g in ((qkv[:, :H], gq), (qkv[:, H:H + K], gk)))
+        ao, _ = R.paged_attention(q, k[None].transpose(0, 2, 1, 3), qkv[None, :, H + K:].transpose(0, 2, 1, 3),
+                                  np.zeros((1, 1), np.int32), [n], [n])
+        h = x + ao.reshape(n, -1) @ w["w_o"]
+        z = rms(h, w["ffn_norm"])
+        gate = z @ w["w_gate"]
+        refs.append(h + (gate / (1 + np.exp(-gate)) * (z @ w["w_up"])) @ w["w_down"])
+    dev = [to_dev(w[n], torch.bfloat16) for n in ("attn_norm", "w_qkv", "w_o", "ffn_norm", "w_gate", "w_up", "w_down")]
+    tab, dgq, dgk = ops.rope_table(max(lens), D), to_dev(gq, torch.bfloat16), to_dev(gk, torch.bfloat16)
+    kc, vc = (torch.full((10, K, page, D), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pt = torch.tensor([[3, 9, 0, 5, 1], [2, 7, 4, -1, -1]], dtype=torch.int32, device="cuda")
+    need = ops.llama_block_paged_workspace_bytes(80, dm, H, K, D, F)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    at, got = [0, 0], [[], []]
+    for step in ((40, 0), (0, 33), (30, 5), (1, 1), (1, 1), (3, 0)):
+        x = np.concatenate([xs[i][at[i]:at[i] + n] for i, n in enumerate(step)])
+        at = [a + n for a, n in zip(at, step)]
+        cu = torch.tensor([0, step[0], sum(step)], dtype=torch.int32, device="cuda")
+        kv = torch.tensor(at, dtype=torch.int32, device="cuda")
+        out = ops.llama_block_paged_fwd(to_dev(x, torch.bfloat16), *dev, kc, vc, pt, cu, kv, H, table=tab, q_gain=dgq,
+                                        k_gain=dgk, max_q=max(step), workspace=ws if step[0] % 2 else None)
+        out = to_np(out)
+        got[0].append(out[:step[0]])
+        got[1].append(out[step[0]:])
+    assert at == list(lens) and ops.device_status(0)[0] == 0
+    for i in range(2):
+        mine = np.concatenate(got[i])
+        assert rel_err(mine, refs[i]) <= BF16_TOL
+        assert rel_err(mine - xs[i], refs[i] - xs[i]) <= BF16_TOL
+
+
 def test_captured_step_follows_the_tables_on_the_device():
     """One captured append + attention, replayed while kv_lens and the inputs change on the device, on a
     side stream with a workspace of its own."""
