@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
   const int tid = (int)threadIdx.x;
   const int ty = tid >> 4, tx = tid & 15;
   pdl_launch_dependents();
+  pdl_wait();
   PagedWalk walk;
   if (warp_id() == 0) {
     walk.start(p, KT, (int)blockIdx.x, (int)gridDim.x);
@@ -310,11 +311,9 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
     const PagedItem x = item;
     const int rows = min(p.rpi, x.q_len * group - x.row0);
     const bool works = (ty & ~1) < rows;  // the warp has a row
-    auto lookup = [&](int j, int buf) {
-      if (tid < KT) {
-        const int key = j * KT + tid;
-        s_off[buf * KT + tid] = j < x.b && key < x.kv ? paged_key(p.pg, x.seq, x.kvh, key) : -1;
-      }
+    auto lookup = [&](int j) -> long long {  // cache offset of key tid of a tile
+      const int key = j * KT + tid;
+      return tid < KT && j < x.b && key < x.kv ? paged_key(p.pg, x.seq, x.kvh, key) : -1;
     };
     auto copy = [&](int buf) {
       for (int e = tid; e < KT * (D / 4); e += 256) {
@@ -339,18 +338,18 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
       }
       cp_async_commit();
     };
-    lookup(x.a, 0);
+    const long long off0 = lookup(x.a);
+    long long off = lookup(x.a + 1);  // of the tile after the one that is copied next
+    if (tid < KT) s_off[tid] = off0;
     __syncthreads();
     copy(0);
-    lookup(x.a + 1, 1);
-    for (int e = tid; e < min(BM, (rows + 15) & ~15) * D; e += 256) {
-      const int r = e / D, d = e % D;
-      float v = 0.0f;
-      if (r < rows) {
-        const int fr = x.row0 + r;
-        v = ldf(q + (long long)(x.q0 + fr / group) * p.q_stride + ((long long)x.kvh * group + fr % group) * D + d);
+    {  // query rows, four threads each
+      const int r = tid >> 2, fr = x.row0 + r;
+      const T* src = q + (long long)(x.q0 + fr / group) * p.q_stride + ((long long)x.kvh * group + fr % group) * D;
+      if (r < ((rows + 15) & ~15)) {
+#pragma unroll 8
+        for (int d = tid & 3; d < D; d += 4) sq[r * LD + d] = r < rows ? ldf(src + d) * p.scale : 0.0f;
       }
-      sq[r * LD + d] = v * p.scale;
     }
     if (tid < BM) {
       s_m[tid] = -INFINITY;
@@ -359,15 +358,16 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
     float o[RT][CT] = {};
     for (int j = x.a; j < x.b; ++j) {
       const int k0 = j * KT, buf = (j - x.a) & 1;
-      __syncthreads();  // the next tile's offsets are there, and its buffer has been used
       if (j + 1 < x.b) {
+        if (tid < KT) s_off[(buf ^ 1) * KT + tid] = off;
+        __syncthreads();  // the next tile's offsets are there, and its buffer has been used
         copy(buf ^ 1);
+        off = lookup(j + 2);
         cp_async_wait<1>();
       } else {
         cp_async_wait<0>();
       }
       __syncthreads();
-      if (j + 2 < x.b) lookup(j + 2, buf);
       if (!works) continue;
       const float* kt = sk + buf * KT * LD;
       const float* vt = sv + buf * KT * LD;
@@ -505,26 +505,40 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
     const int r = (block - first[c]) * 32 + lane, rows = h.w & 0xffff;
     const PagedPieces pc{c, h.w >> 16};
     if (r >= rows) continue;
-    float mx = -INFINITY;
-#pragma unroll 8
-    for (int i = 0; i < pc.n; ++i) mx = fmaxf(mx, p.part_ml[pc.slot(i) * p.rpi + r].x);
-    const float base = mx == -INFINITY ? 0.0f : mx;
-    float l = 0.0f, o[16] = {};
-#pragma unroll 4
-    for (int i = 0; i < pc.n; ++i) {
-      const float2 ml = p.part_ml[pc.slot(i) * p.rpi + r];
-      // a piece without a key of this row has left old values in its slot: read all the same, so that no
-      // load waits for another, and passed over
-      const bool have = ml.x != -INFINITY;
-      const float wgt = have ? exp2f(ml.x - base) : 0.0f;
-      l = fmaf(ml.y, wgt, l);
+    // one pass over the pieces with a running maximum, four pieces' loads at a time.  A piece without a
+    // key of this row has left old values in its slot: read all the same, so that no load waits for
+    // another, and passed over.
+    float mx = -INFINITY, l = 0.0f, o[16] = {};
+    for (int i0 = 0; i0 < pc.n; i0 += 4) {
+      float2 ml[4];
+      float4 v[4][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 v = *paged_part(p, pc.slot(i), c0 + q, r);
-        o[4 * q] = have ? fmaf(v.x, wgt, o[4 * q]) : o[4 * q];
-        o[4 * q + 1] = have ? fmaf(v.y, wgt, o[4 * q + 1]) : o[4 * q + 1];
-        o[4 * q + 2] = have ? fmaf(v.z, wgt, o[4 * q + 2]) : o[4 * q + 2];
-        o[4 * q + 3] = have ? fmaf(v.w, wgt, o[4 * q + 3]) : o[4 * q + 3];
+      for (int i = 0; i < 4; ++i) {
+        const long long slot = pc.slot(min(i0 + i, pc.n - 1));
+        ml[i] = p.part_ml[slot * p.rpi + r];
+        if (i0 + i >= pc.n) ml[i].x = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[i][q] = *paged_part(p, slot, c0 + q, r);
+      }
+      const float m_new = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), mx);
+      if (m_new == -INFINITY) continue;
+      const float alpha = exp2f(mx - m_new);
+      mx = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] *= alpha;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (ml[i].x == -INFINITY) continue;
+        const float wgt = exp2f(ml[i].x - mx);
+        l = fmaf(ml[i].y, wgt, l);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          o[4 * q] = fmaf(v[i][q].x, wgt, o[4 * q]);
+          o[4 * q + 1] = fmaf(v[i][q].y, wgt, o[4 * q + 1]);
+          o[4 * q + 2] = fmaf(v[i][q].z, wgt, o[4 * q + 2]);
+          o[4 * q + 3] = fmaf(v[i][q].w, wgt, o[4 * q + 3]);
+        }
       }
     }
     const int fr = h.z + r;
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
 #pragma unroll
       for (int e = 0; e < 16; ++e) stf(dst + e, o[e]);
     }
-    if (c0 == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? (base + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    if (c0 == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? (mx + log2f(l)) * 0.69314718055994531f : -INFINITY;
   }
 }
 
