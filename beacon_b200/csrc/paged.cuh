@@ -44,11 +44,6 @@ enum : unsigned int {
   kSitePagedMerge = 0x613,
 };
 
-// Programmatic dependent launch: the join is launched while the attention kernel runs and waits here
-// for all of its results.
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // One contiguous piece of an item: tiles [a, b) of its n.
 struct PagedItem {
   int seq, kvh, row0;  // first row within the sequence's R

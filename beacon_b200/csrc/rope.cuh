@@ -76,17 +76,28 @@ struct TokenPlace {
   int b, s;        // head-major form: batch entry and place in the sequence
   long long slot;  // paged form: cache offset of (page, head 0, token), -1: nowhere
 };
+// The sequence that the last token belonged to: a warp's tokens ascend, and in a prompt the next one is
+// mostly of the same sequence, so that only its page is left to look up.
+struct TokenSeq {
+  int s = -1, first = 0, end = 0, kv = 0;
+};
 template <bool PAGED>
-__device__ __forceinline__ TokenPlace token_place(const RopeParams& p, int t) {
+__device__ __forceinline__ TokenPlace token_place(const RopeParams& p, int t, TokenSeq& q) {
   TokenPlace w{true, 0, 0, 0, -1};
   if constexpr (PAGED) {
     const PagedSeqs& g = p.pg;
-    const int s = warp_owner(g.cu_q, g.seqs, t);
-    if (s >= g.seqs || t < __ldg(g.cu_q)) {
-      w.on = false;
-      return w;
+    if (q.s < 0 || t < q.first || t >= q.end) {
+      q.s = warp_owner(g.cu_q, g.seqs, t);
+      if (q.s >= g.seqs || t < __ldg(g.cu_q)) {
+        q.s = -1;
+        w.on = false;
+        return w;
+      }
+      q.first = __ldg(g.cu_q + q.s);
+      q.end = __ldg(g.cu_q + q.s + 1);
+      q.kv = __ldg(g.kv_lens + q.s);
     }
-    const int at = __ldg(g.kv_lens + s) - (__ldg(g.cu_q + s + 1) - t);
+    const int s = q.s, at = q.kv - (q.end - t);
     w.pos = at;
     if (at >= 0) {
       const int pi = (int)((unsigned)at / (unsigned)g.page_size);
@@ -151,7 +162,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_any(T* __restrict__ q, T* 
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
     const long long t = u / heads;
     const int h = (int)(u - t * heads);
-    const TokenPlace w = token_place<PAGED>(p, (int)t);
+    TokenSeq seq;
+    const TokenPlace w = token_place<PAGED>(p, (int)t, seq);
     if (!w.on) continue;
     const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
     T* o = head_out<T, PAGED>(p, w, (int)t, kind, kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv, q, k, v);
@@ -193,6 +205,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
                                                               const T* __restrict__ q_gain,
                                                               const T* __restrict__ k_gain, const RopeParams p) {
   __shared__ float red[8][kRopeMaxDim];
+  pdl_launch_dependents();
   const int lane = (int)lane_id(), warp = (int)warp_id();
   const int heads = p.Hq + 2 * p.Hkv;
   const long long n = p.tokens * heads, warps = (long long)gridDim.x * (blockDim.x >> 5);
@@ -200,7 +213,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
     const long long t = u / heads;
     const int h = (int)(u - t * heads);
-    const TokenPlace w = token_place<false>(p, (int)t);
+    TokenSeq seq;
+    const TokenPlace w = token_place<false>(p, (int)t, seq);
     const int kind = h < p.Hq ? 0 : h < p.Hq + p.Hkv ? 1 : 2;
     const T* dy = head_out<const T, false>(p, w, (int)t, kind, kind == 0 ? h : kind == 1 ? h - p.Hq : h - p.Hq - p.Hkv, dq,
                                            dk, dv);
@@ -553,11 +567,12 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, 
     ldraw(gain + ln.e1, g1);
   }
   int stage = 0;
+  TokenSeq seq;
   for (long long t = w.t0; t < p.tokens; t += w.step) {
     fetch(t + (long long)(kRopeStages - 1) * w.step, stage == 0 ? kRopeStages - 1 : stage - 1);
     const int at = stage;
     stage = stage + 1 == kRopeStages ? 0 : stage + 1;
-    const TokenPlace pl = token_place<PAGED>(p, (int)t);
+    const TokenPlace pl = token_place<PAGED>(p, (int)t, seq);
     RopeMap map;
     if (w.kind != 2) {
       float c[8], s[8], ga[8], gz[8];
@@ -623,6 +638,7 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
   extern __shared__ __align__(16) uint8_t rope_smem[];
   __shared__ float red[8][D];
   __shared__ int kinds[8];
+  pdl_launch_dependents();
   const RopeLane<D> ln(p.rot);
   const RopeWork<D, U> w(p, nb, ln.sub);
   const RopeStage<T, 4 * U> st(rope_smem, (int)warp_id());
@@ -660,11 +676,12 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
   }
   float acc0[8] = {}, acc1[8] = {};
   int stage = 0;
+  TokenSeq seq;
   for (long long t = w.t0; t < last; t += w.step) {
     fetch(t + (long long)(kRopeStages - 1) * w.step, stage == 0 ? kRopeStages - 1 : stage - 1);
     const int at = stage;
     stage = stage + 1 == kRopeStages ? 0 : stage + 1;
-    const TokenPlace pl = token_place<false>(p, (int)t);
+    const TokenPlace pl = token_place<false>(p, (int)t, seq);
     float c[8], s[8];
     if (w.kind != 2) ln.turn(p, pl.pos, c, s);
     cp_async_wait<kRopeStages - 1>();
@@ -746,6 +763,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_rope_gain_sum(T* __restrict__ dq_gain, T* __restrict__ dk_gain,
                                                        const float* __restrict__ part, int nparts, int D) {
   __shared__ float red[8][32];
+  pdl_wait();
   T* out = blockIdx.x == 0 ? dq_gain : dk_gain;
   if (out == nullptr) return;
   const int lane = (int)lane_id(), warp = (int)warp_id(), d = (int)blockIdx.y * 32 + lane;

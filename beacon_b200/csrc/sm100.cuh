@@ -444,6 +444,11 @@ __device__ __forceinline__ void umma_commit_leader(uint64_t* bar) {
                : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched that way may be resident before the one ahead of it on its
+// stream has ended (once all of that one's CTAs have allowed it or are done) and waits here for its results.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Named barrier among `nthreads` threads (multiple of 32).
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
