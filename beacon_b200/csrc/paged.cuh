@@ -470,6 +470,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int runs) {
   __shared__ int4 heads[kPagedMostRuns];
   __shared__ int first[kPagedMostRuns + 1];  // 32-row blocks of the items before
+  pdl_launch_dependents();
   pdl_wait();
   const int lane = (int)lane_id();
   for (int c = (int)threadIdx.x; c < runs; c += 256) heads[c] = p.heads[c];

@@ -159,6 +159,8 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_any(T* __restrict__ q, T* 
   const int lane = (int)lane_id();
   const int heads = p.Hq + 2 * p.Hkv;
   const long long n = p.tokens * heads, warps = (long long)gridDim.x * (blockDim.x >> 5);
+  pdl_launch_dependents();
+  pdl_wait();
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < n; u += warps) {
     const long long t = u / heads;
     const int h = (int)(u - t * heads);
@@ -206,6 +208,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
                                                               const T* __restrict__ k_gain, const RopeParams p) {
   __shared__ float red[8][kRopeMaxDim];
   pdl_launch_dependents();
+  pdl_wait();
   const int lane = (int)lane_id(), warp = (int)warp_id();
   const int heads = p.Hq + 2 * p.Hkv;
   const long long n = p.tokens * heads, warps = (long long)gridDim.x * (blockDim.x >> 5);
@@ -543,7 +546,9 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, 
   extern __shared__ __align__(16) uint8_t rope_smem[];
   const RopeLane<D> ln(p.rot);
   const RopeWork<D, U> w(p, nb, ln.sub);
+  pdl_launch_dependents();
   if (!w.on) return;
+  pdl_wait();
   const RopeStage<T, 2 * U> st(rope_smem, (int)warp_id());
   const T* gain = w.kind == 0 ? q_gain : w.kind == 1 ? k_gain : nullptr;
   auto fetch = [&](long long t, int stage) {  // 64 bits: t runs past the last token
@@ -639,6 +644,7 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
   __shared__ float red[8][D];
   __shared__ int kinds[8];
   pdl_launch_dependents();
+  pdl_wait();
   const RopeLane<D> ln(p.rot);
   const RopeWork<D, U> w(p, nb, ln.sub);
   const RopeStage<T, 4 * U> st(rope_smem, (int)warp_id());
@@ -763,6 +769,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_rope_gain_sum(T* __restrict__ dq_gain, T* __restrict__ dk_gain,
                                                        const float* __restrict__ part, int nparts, int D) {
   __shared__ float red[8][32];
+  pdl_launch_dependents();
   pdl_wait();
   T* out = blockIdx.x == 0 ? dq_gain : dk_gain;
   if (out == nullptr) return;
