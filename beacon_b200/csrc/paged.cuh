@@ -104,9 +104,7 @@ struct PagedWalk {
     int total = w0;
 #pragma unroll 1
     for (int s = lane + 32; s < p.pg.seqs; s += 32) total += paged_seq_work(p, s, kt);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= p.Hkv;
+    total = __reduce_add_sync(0xffffffffu, total) * p.Hkv;
     chunk = max(1, (int)(((unsigned)total + (unsigned)runs - 1u) / (unsigned)runs));
     int at = (int)min((unsigned)run * (unsigned)chunk, (unsigned)total);
     left = min(chunk, total - at);
@@ -214,18 +212,21 @@ __device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x, int chun
 constexpr int kPagedMaxRuns = 160, kPagedParts = 16;
 __device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns][kPagedParts];
 
-// One warp, after its part of a piece has been written: whether that part of every piece now has been.
+// One warp, after its part of a piece has been written: whether that part of every piece now has been.  One
+// lane's release-acquire add stands for the warp, ordered with the others' accesses by the warp
+// barriers around it (a fence in every lane and a relaxed add took twice as long).
 __device__ __forceinline__ bool paged_last_piece(int slot, const PagedPieces& pc, int part) {
-  __threadfence();
   __syncwarp();
   unsigned int last = 0u;
   if (lane_id() == 0) {
     unsigned int* done = &g_paged_done[slot][pc.first][part];
-    last = atomicAdd(done, 1u) == (unsigned int)pc.n - 1u ? 1u : 0u;
-    if (last) atomicExch(done, 0u);
+    unsigned int before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(done) : "memory");
+    last = before == (unsigned int)pc.n - 1u ? 1u : 0u;
+    if (last) *reinterpret_cast<volatile unsigned int*>(done) = 0u;  // for the launch that takes the set next
   }
   last = __shfl_sync(0xffffffffu, last, 0);
-  if (last) __threadfence();
+  __syncwarp();
   return last != 0u;
 }
 

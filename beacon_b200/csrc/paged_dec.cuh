@@ -135,10 +135,6 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
     cp_async_commit();
     fstage = fstage + 1 == kDecStages ? 0 : fstage + 1;
   };
-  seek();
-#pragma unroll 1
-  for (int s = 0; s < kDecStages - 1; ++s) fetch();
-
   // query rows of this thread: lane / 4 and lane / 4 + 8 of the item
   uint32_t qf[D / 16][4];
   int lim[2];
@@ -176,9 +172,16 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   PagedItem x;
   int stage = 0;
   uint32_t merges = 0;
+  bool primed = false;
 #pragma unroll 1
   while (walk.next(p, kDecKt, x)) {
-    load_q(x);  // its latency is covered by the copies in flight
+    load_q(x);  // used after the first keys have come
+    if (!primed) {
+      primed = true;
+      seek();
+#pragma unroll 1
+      for (int s = 0; s < kDecStages - 1; ++s) fetch();
+    }
     float o[D / 8][4] = {};
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     const int steps = steps_of(x);
@@ -303,6 +306,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
       for (int e = 0; e < CPL; ++e) po[e] = ot[e];
       if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);
       if (!paged_last_piece(p.sched_slot, pc, r)) continue;
+      // lane i weighs piece i (of 32 at a time); the pieces' rows then load side by side
       mx = -INFINITY;
       for (int i = lane; i < pc.n; i += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);
 #pragma unroll
@@ -311,23 +315,30 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
       lt = 0.0f;
 #pragma unroll
       for (int e = 0; e < CPL; ++e) ot[e] = 0.0f;
-#pragma unroll 4
-      for (int i = 0; i < pc.n; ++i) {
-        const long long at = pc.slot(i) * p.rpi + r;
-        const float2 ml = __ldcg(&p.part_ml[at]);
-        const float wgt = ex2_approx(ml.x - base);
-        lt = fmaf(ml.y, wgt, lt);
-        const float* src = p.part_o + at * D + CPL * lane;
-        if constexpr (CPL == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          ot[0] = fmaf(v.x, wgt, ot[0]);
-          ot[1] = fmaf(v.y, wgt, ot[1]);
-          ot[2] = fmaf(v.z, wgt, ot[2]);
-          ot[3] = fmaf(v.w, wgt, ot[3]);
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          ot[0] = fmaf(v.x, wgt, ot[0]);
-          ot[1] = fmaf(v.y, wgt, ot[1]);
+#pragma unroll 1
+      for (int i0 = 0; i0 < pc.n; i0 += 32) {
+        const float2 ml = i0 + lane < pc.n ? __ldcg(&p.part_ml[pc.slot(i0 + lane) * p.rpi + r])
+                                           : make_float2(-INFINITY, 0.0f);
+        const float wl = ex2_approx(ml.x - base);
+        lt += warp_sum(wl * ml.y);
+        const int n = min(32, pc.n - i0);
+#pragma unroll 1
+        for (int i1 = 0; i1 < n; i1 += 8) {
+          float v[8][CPL];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float* src = p.part_o + (pc.slot(i0 + min(i1 + i, n - 1)) * p.rpi + r) * D + CPL * lane;
+            if constexpr (CPL == 4) *reinterpret_cast<float4*>(v[i]) = __ldcg(reinterpret_cast<const float4*>(src));
+            else *reinterpret_cast<float2*>(v[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float wgt = __shfl_sync(0xffffffffu, wl, min(i1 + i, 31));
+            if (i1 + i < n) {
+#pragma unroll
+              for (int e = 0; e < CPL; ++e) ot[e] = fmaf(v[i][e], wgt, ot[e]);
+            }
+          }
         }
       }
       store_row(x, r, mx, lt, ot);
