@@ -9,7 +9,10 @@
 // zeros.  The slots between the last key and the end of its box may hold anything: the masked S
 // columns are replaced, and the MMA warp overwrites those V rows with zeros before the tile's PV.
 //
-//   warp 0      producer (whole warp): the run's items (published in a ring), Q tiles, K and V rings
+//   warp 0      producer (whole warp): the run's items (published in a ring), Q tiles, K ring
+//   warp 2      producer of the V ring.  One producer of both let K(j+2) wait for the V stage that PV(j-1)
+//               frees, so that a tile's S came late: 64 sequences of 500-8192 keys, 8 new tokens each,
+//               32/8 heads of 128: 247 us with one, 153 us with two.
 //   warp 1      TMEM allocator, MMA issuer:  S_A S_B | O_A += P_A V, S_A', O_B += P_B V, S_B' | ...
 //   warps 4-7   softmax of tile A, warps 8-11 of tile B: one row per thread, fp32 statistics, P (bf16)
 //               back into the S region of TMEM, O rescaled there when the maximum grows by over 2^8.
@@ -58,11 +61,12 @@ enum : unsigned int {
 };
 
 constexpr int kPtcItems = 4;  // items published ahead
-// An item's start and end against a key tile: 1 to 3 measured alike (0: 20% slower at 32-token chunks).
-constexpr int kPtcItemCost = 2;
+// An item's start and end against a key tile (16 sequences of 1-512 new tokens after 100-7500: cost 0 138 us,
+// 1 119 us, 2 112 us, 4 110 us; 64 sequences of 1-40 new tokens: 169, 143, 135, 130 us).
+constexpr int kPtcItemCost = 4;
 struct PtcItem {
   int valid;
-  int kvh, tok0;       // KV head; first token row of the item in q
+  int seq, kvh, tok0;  // sequence; KV head; first token row of the item in q
   int ntok;            // tokens from tok0 to the sequence's end
   int lim0;            // keys that token tok0 sees (tok0 + i: lim0 + i), or kv when not causal
   int kv;
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* dual_full = drain + 1;               // [4] per 32 rows: B's rows of a dual item are written
   uint64_t* dual_free = dual_full + 4;           // [4] A has read them
   uint64_t* item_full = dual_free + 4;           // [kPtcItems]
-  uint64_t* item_empty = item_full + kPtcItems;  // [kPtcItems] read by the MMA warp and 8 softmax warps
+  uint64_t* item_empty = item_full + kPtcItems;  // [kPtcItems] read by the MMA warp, the V producer and 8 softmax warps
   PtcItem* items = reinterpret_cast<PtcItem*>(item_empty + kPtcItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPtcItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(384, 1)
     }
     for (int i = 0; i < kPtcItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 9);
+      mbar_init(&item_empty[i], 10);
     }
     *abort_flag = 0;
     fence_mbarrier_init();
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(384, 1)
       walk.start(p, 128, (int)blockIdx.x, (int)gridDim.x);
       const int nbox = 128 / tp.box;
       const uint32_t q_tile_bytes = (uint32_t)(tp.tpt * p.g) * 128u * (D / 64);
-      uint32_t tk = 0, kissued = 0, vissued = 0, kpar = 0, vpar = 0, qissued = 0, qpar = 0;
+      uint32_t tk = 0, kissued = 0, kpar = 0, qissued = 0, qpar = 0;
       bool ok = true;
       for (int ci = 0; ok; ++ci) {
         PagedItem w{};
@@ -253,21 +257,22 @@ __global__ void __launch_bounds__(384, 1)
         x.valid = more ? 1 : 0;
         if (more) {
           const int t0 = w.row0 / p.g;
+          x.seq = w.seq;
           x.kvh = w.kvh;
           x.tok0 = w.q0 + t0;
           x.ntok = w.q_len - t0;
           x.lim0 = p.causal ? w.kv - w.q_len + t0 + 1 : w.kv;
           x.kv = w.kv;
+          x.slot = (w.a == 0 && w.b == w.n) ? -1 : paged_slot(w);
           x.a = w.a;
           x.b = w.b;
-          x.slot = (w.a == 0 && w.b == w.n) ? -1 : paged_slot(w);
           x.pieces = paged_pieces(w, walk.chunk);
           x.dual = x.ntok <= tp.tpt ? 1 : 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int last = min((t + 1) * tp.tpt, x.ntok) - 1;
             const int keys = p.causal ? max(0, x.lim0 + last) : x.kv;
-            x.end[t] = t * tp.tpt < x.ntok ? min(w.b, max(1, (keys + 127) / 128)) : 0;
+            x.end[t] = t * tp.tpt < x.ntok ? min(x.b, max(1, (keys + 127) / 128)) : 0;
           }
         }
         const int is = ci % kPtcItems;
@@ -309,6 +314,32 @@ __global__ void __launch_bounds__(384, 1)
           }
           kissued |= 1u << st;
           kpar = (kpar & ~(1u << st)) | (ph << st);
+        }
+      }
+      if (!ok && lane == 0) {  // a wait gave up: the copies in flight land before the CTA may end
+        volatile int no_abort = 0;
+        if (qissued) mbar_wait(q_full, qpar, &no_abort, kSitePtcDrain);
+        for (int s = 0; s < ST; ++s) {
+          if (kissued & (1u << s)) mbar_wait(&k_full[s], (kpar >> s) & 1u, &no_abort, kSitePtcDrain);
+        }
+      }
+    } else if (warp == 2) {
+      // -------------------------------------------------------------- V producer
+      const int nbox = 128 / tp.box;
+      uint32_t tk = 0, vissued = 0, vpar = 0;
+      bool ok = true;
+      PtcItem x;
+      for (int ci = 0; ok; ++ci) {
+        const bool got = read_item(ci, x);
+        if (!__all_sync(0xffffffffu, got)) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[ci % kPtcItems]);
+        int page = (int)lane < nbox ? ptc_page(p.pg, x.seq, x.a * 128 + (int)lane * tp.box, x.kv) : 0;
+        for (int j = x.a; j < x.b; ++j, ++tk) {
+          const uint32_t st = tk & (ST - 1), ph = (tk >> LOG) & 1u;
+          const int key = j * 128 + (int)lane * tp.box, cur = page;
+          if (j + 1 < x.b && (int)lane < nbox) page = ptc_page(p.pg, x.seq, key + 128, x.kv);
+          const int row = key % p.pg.page_size;
           ok = warp_wait(&v_empty[st], ph ^ 1u, abort_flag, kSitePtcKv);
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(&v_full[st], Cfg::KV_BYTES);
@@ -323,13 +354,10 @@ __global__ void __launch_bounds__(384, 1)
           vpar = (vpar & ~(1u << st)) | (ph << st);
         }
       }
-      if (!ok && lane == 0) {  // a wait gave up: the copies in flight land before the CTA may end
+      if (!ok && lane == 0) {
         volatile int no_abort = 0;
-        if (qissued) mbar_wait(q_full, qpar, &no_abort, kSitePtcDrain);
-        for (int s = 0; s < ST; ++s) {
-          if (kissued & (1u << s)) mbar_wait(&k_full[s], (kpar >> s) & 1u, &no_abort, kSitePtcDrain);
+        for (int s = 0; s < ST; ++s)
           if (vissued & (1u << s)) mbar_wait(&v_full[s], (vpar >> s) & 1u, &no_abort, kSitePtcDrain);
-        }
       }
     } else if (warp == 1) {
       // -------------------------------------------------------------- MMA issuer
