@@ -20,7 +20,7 @@
 //
 // An item whose rows fit tile A is `dual`: B takes the same query tile over every other key tile, so
 // that one tile's softmax still runs beside the other's products (a lone tile's chain of S, softmax
-// and PV measured 2.2 us per 128 keys); at its end B's rows go to A through the workspace.  The rows
+// and PV measured 2.2 us per 128 keys); at its end each of the two takes half of the columns.  The rows
 // of an item in two pieces are joined by the warp that finishes the second one; k_paged_join joins
 // those of items in more (one warp that reads 16 pieces took 45 us, the whole device a few).
 //
@@ -37,7 +37,7 @@ struct PagedTcCfg {
   static constexpr uint32_t Q_BYTES = 128 * D * 2;
   static constexpr uint32_t KV_BYTES = 128 * D * 2;
   static constexpr int STAGES = D == 64 ? 4 : 2;  // K and V tiles in flight: 64 KB each
-  static constexpr size_t SMEM_BYTES = 1024 + 2 * (size_t)Q_BYTES + 2 * STAGES * (size_t)KV_BYTES + 1024;
+  static constexpr size_t SMEM_BYTES = 1024 + 2 * (size_t)Q_BYTES + 2 * STAGES * (size_t)KV_BYTES + 1024 + 256 * sizeof(float2);
   static constexpr int THREADS = 384;
 };
 
@@ -176,16 +176,15 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* o_full = p_full + 4;    // [2]
   uint64_t* clean = o_full + 2;     // the MMA warp's lanes have zeroed a V tile's tail
   uint64_t* drain = clean + 1;
-  uint64_t* dual_full = drain + 1;               // [4] per 32 rows: B's rows of a dual item are written
-  uint64_t* dual_free = dual_full + 4;           // [4] A has read them
+  uint64_t* dual_full = drain + 1;               // [4] per 32 rows of a dual item: A's and B's sums are final
+  uint64_t* dual_free = dual_full + 4;           // [4] both have read the other's
   uint64_t* item_full = dual_free + 4;           // [kPtcItems]
   uint64_t* item_empty = item_full + kPtcItems;  // [kPtcItems] read by the MMA warp, the V producer and 8 softmax warps
   PtcItem* items = reinterpret_cast<PtcItem*>(item_empty + kPtcItems);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + kPtcItems);
+  float2* dual_ml = reinterpret_cast<float2*>(items + kPtcItems);  // [2][128] a dual item's (m, l)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dual_ml + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t warp = warp_id(), lane = lane_id();
-  // rows that B hands to A in dual items: one extra slot per CTA
-  const long long dual_slot = 2LL * gridDim.x + blockIdx.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
@@ -205,8 +204,8 @@ __global__ void __launch_bounds__(384, 1)
     mbar_init(clean, 32);
     mbar_init(drain, 1);
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&dual_full[i], 1);
-      mbar_init(&dual_free[i], 1);
+      mbar_init(&dual_full[i], 2);
+      mbar_init(&dual_free[i], 2);
     }
     for (int i = 0; i < kPtcItems; ++i) {
       mbar_init(&item_full[i], 1);
@@ -580,58 +579,48 @@ __global__ void __launch_bounds__(384, 1)
           dst[(long long)e * p.rpi] = make_float4(__uint_as_float(u[4 * e]), __uint_as_float(u[4 * e + 1]),
                                                   __uint_as_float(u[4 * e + 2]), __uint_as_float(u[4 * e + 3]));
       };
-      float w_own = 1.0f, w_other = 0.0f;  // dual: weights of A's and B's rows in their sum
-      const float4* other = nullptr;
+      // Dual: a row's two threads (same lanes of TMEM) hold sums over alternate key tiles.  Their statistics
+      // cross through shared memory; then each finishes half of the row's columns.
+      const uint32_t qd = warp & 3u;
+      float w_a = 1.0f, w_b = 0.0f;
+      int c0 = 0, c1 = D / 32;
       if (x.dual) {
-        if (x.b - x.a == 1) {
-          if (t == 1) continue;  // one key tile: A alone
-        } else {
-          const long long row = dual_slot * p.rpi + r;
-          float4* po = paged_part(p, dual_slot, 0, r);
-          const uint32_t use = duals++, qd = warp & 3u;
-          if (t == 1) {
-            ok = warp_wait(&dual_free[qd], (use & 1u) ^ 1u, abort_flag, kSitePtcDual);
-            if (!ok) break;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t u[32];
-              tmem_ld32(tmem + lane_base + o_col + c * 32, u);
-              tmem_wait_ld();
-              if (row_ok) store_part(po + (long long)(8 * c) * p.rpi, u);
-            }
-            if (row_ok) p.part_ml[row] = make_float2(m_used, l);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&dual_full[qd]);
-            continue;
-          }
-          ok = warp_wait(&dual_full[qd], use & 1u, abort_flag, kSitePtcDual);
-          if (!ok) break;
-          if (row_ok) {
-            const float2 ml = __ldcg(&p.part_ml[row]);
-            const float mx = fmaxf(m_used, ml.x);
-            const float base = mx == -INFINITY ? 0.0f : mx;
-            w_own = ex2_approx(m_used - base);
-            w_other = ex2_approx(ml.x - base);
-            l = l * w_own + ml.y * w_other;
-            m_used = mx;
-            other = po;
-          }
-        }
+        dual_ml[t * 128 + r] = make_float2(m_used, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dual_full[qd]);
+        ok = warp_wait(&dual_full[qd], duals & 1u, abort_flag, kSitePtcDual);
+        if (!ok) break;
+        tc_fence_after();
+        const float2 ml = dual_ml[(1 - t) * 128 + r];
+        const float mx = fmaxf(m_used, ml.x);
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float w_own = ex2_approx(m_used - base), w_other = ex2_approx(ml.x - base);
+        w_a = t == 0 ? w_own : w_other;
+        w_b = t == 0 ? w_other : w_own;
+        l = t == 0 ? fmaf(l, w_a, ml.y * w_b) : fmaf(ml.y, w_a, l * w_b);  // the same sum on both sides
+        m_used = mx;
+        c0 = t * (D / 64);
+        c1 = c0 + D / 64;
       }
+      const bool has = x.dual || count > 0;  // the tile saw keys of this piece
       // columns [32 c, 32 c + 32) of the row's O, relative to m_used (whole warp)
       auto load_o = [&](int c, uint32_t (&u)[32]) {
-        tmem_ld32(tmem + lane_base + o_col + c * 32, u);
-        tmem_wait_ld();
-        if (other != nullptr) {
+        if (!x.dual) {
+          tmem_ld32(tmem + lane_base + o_col + c * 32, u);
+          tmem_wait_ld();
+          return;
+        }
+        tmem_ld32(tmem + lane_base + 256 + c * 32, u);
+        if (x.b - x.a > 1) {
+          uint32_t ub[32];
+          tmem_ld32(tmem + lane_base + 256 + D + c * 32, ub);
+          tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 v = __ldcg(other + (long long)(8 * c + e / 4) * p.rpi);
-            u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), w_own, v.x * w_other));
-            u[e + 1] = __float_as_uint(fmaf(__uint_as_float(u[e + 1]), w_own, v.y * w_other));
-            u[e + 2] = __float_as_uint(fmaf(__uint_as_float(u[e + 2]), w_own, v.z * w_other));
-            u[e + 3] = __float_as_uint(fmaf(__uint_as_float(u[e + 3]), w_own, v.w * w_other));
-          }
+          for (int e = 0; e < 32; ++e)
+            u[e] = __float_as_uint(fmaf(__uint_as_float(u[e]), w_a, __uint_as_float(ub[e]) * w_b));
+        } else {
+          tmem_wait_ld();  // A alone has had a key tile
         }
       };
       const long long at = (long long)(x.tok0 + tok) * p.Hq + (long long)x.kvh * p.g + head;
@@ -654,23 +643,27 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       };
+      const bool any_row = __any_sync(0xffffffffu, row_ok);
+      const bool lse_row = p.lse != nullptr && !(x.dual && t == 1);
       if (x.slot < 0) {
-        if (count == 0) continue;  // a tile B without rows
+        if (!has) continue;  // a tile B without rows
         const bool none = m_used == -INFINITY;
         const float inv = none ? 0.0f : 1.0f / l;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = c0; c < c1 && any_row; ++c) {
           uint32_t u[32];
           load_o(c, u);
           if (row_ok) store_o(c, u, inv, none);
         }
-        if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
-      } else if (__any_sync(0xffffffffu, row_ok)) {
+        if (row_ok && lse_row) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
+      } else if (any_row) {
         const int row = (x.dual ? 0 : t * tp.tpt * p.g) + r;  // row of the item
-        const long long own = (long long)x.slot * p.rpi + row;
-        if (count > 0) {
+        // statistics of the row; B keeps its own copy of a dual item's, in rows that the item does not have
+        const int ml_row = row + (x.dual ? t * tp.tpt * p.g : 0);
+        const long long own = (long long)x.slot * p.rpi + ml_row;
+        if (has) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = c0; c < c1; ++c) {
             uint32_t u[32];
             load_o(c, u);
             if (row_ok) store_part(paged_part(p, x.slot, 8 * c, row), u);
@@ -681,21 +674,21 @@ __global__ void __launch_bounds__(384, 1)
         if (x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4)) {
           const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second
           const long long that = x.pieces.slot(1 - mine);
-          const float2 ml = row_ok ? __ldcg(&p.part_ml[that * p.rpi + row]) : make_float2(-INFINITY, 0.0f);
+          const float2 ml = row_ok ? __ldcg(&p.part_ml[that * p.rpi + ml_row]) : make_float2(-INFINITY, 0.0f);
           const float mx = fmaxf(m_used, ml.x);
           const bool none = mx == -INFINITY, read = row_ok && ml.x != -INFINITY;
           const float base = none ? 0.0f : mx;
           const float w_mine = ex2_approx(m_used - base), w_that = ex2_approx(ml.x - base);
           const float lt = mine ? fmaf(l, w_mine, ml.y * w_that) : fmaf(ml.y, w_that, l * w_mine);
           const float inv = none ? 0.0f : 1.0f / lt;
-          const float4* src = paged_part(p, that, 0, row);
+          const float4* src = paged_part(p, that, 8 * c0, row);
           float4 v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)e * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = c0; c < c1; ++c) {
             uint32_t u[32];
-            if (count > 0) {
+            if (has) {
               load_o(c, u);
             } else {
 #pragma unroll
@@ -707,20 +700,24 @@ __global__ void __launch_bounds__(384, 1)
               const float a = __uint_as_float(u[e]);
               u[e] = __float_as_uint(mine ? fmaf(a, w_mine, f[e] * w_that) : fmaf(f[e], w_that, a * w_mine));
             }
-            if (c + 1 < D / 32) {
+            if (c + 1 < c1) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)(8 * (c + 1) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)(8 * (c + 1 - c0) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             if (row_ok) store_o(c, u, inv, none);
           }
-          if (row_ok && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (mx + __log2f(lt)) * 0.69314718055994531f;
+          if (row_ok && lse_row) p.lse[at] = none ? -INFINITY : (mx + __log2f(lt)) * 0.69314718055994531f;
         }
         __syncwarp();
       }
       tc_fence_before();
-      if (x.dual && x.b - x.a > 1) {
+      if (x.dual) {  // the other tile's thread has read this one's O and statistics
         __syncwarp();
-        if (lane == 0) mbar_arrive(&dual_free[warp & 3u]);
+        if (lane == 0) mbar_arrive(&dual_free[qd]);
+        ok = warp_wait(&dual_free[qd], duals & 1u, abort_flag, kSitePtcDual);
+        if (!ok) break;
+        ++duals;
+        tc_fence_after();
       }
     }
   }
