@@ -6,14 +6,14 @@
 //   out = softmax(q k^T / sqrt(D)) v, lse = log sum exp; no key visible: out = 0, lse = -inf.
 // For one KV head the rows are (token, query head of the group), token-major: R = q_len * g.
 //
-// Work: an item is `rpi` consecutive rows of one (sequence, KV head); its length is the number of
-// 128- (or 64-) key tiles its last row sees, at least one, behind `item_cost` tiles' worth of time for
-// its start and end.  All items laid end to end (sequence, KV head, item, tile) are cut into gridDim.x
-// equal runs, one per CTA, so that one long context fills the GPU as well as many short ones and the
-// SMs finish together.  A run's first and
-// last item may be partial: their unnormalised rows (O, m, l) go to two workspace slots of the CTA
-// and k_paged_join adds them up in tile order, so results do not depend on timing.  Every CTA finds
-// its run itself from cu_q and kv_lens (one warp, 32 sequences per step): no plan, no host copy.
+// Work: an item is `rpi` consecutive rows of one (sequence, KV head); its length is the time of the
+// 128- (or 64-) key tiles its last row sees, at least one, behind `item_cost` for its start and end.
+// All items laid end to end (sequence, KV head, item, tile) are cut into gridDim.x equal runs, one per
+// CTA, so that one long context fills the GPU as well as many short ones and the SMs finish together; a
+// tile is of the run that holds its end.  A run's first and last item may be partial: their unnormalised
+// rows (O, m, l) go to two workspace slots of the CTA and are added up in tile order, so results do not
+// depend on timing.  Every CTA finds its run itself from cu_q and kv_lens (one warp, 32 sequences per
+// step): no plan, no host copy.
 #pragma once
 
 #include "rope.cuh"
@@ -26,7 +26,8 @@ struct PagedParams {
   int Hq, Hkv, D, g;         // g = Hq / Hkv
   int causal;
   int rpi;                   // rows per item
-  int item_cost;             // time of an item's start and end, in tiles
+  int item_cost;             // time of an item's start and end
+  int half_rows;             // items of at most so many rows take HW, not W, per tile
   float scale;               // 1 / sqrt(D)
   long long q_stride;        // elements between token rows of q
   long long tokens;
@@ -49,15 +50,16 @@ struct PagedItem {
   int seq, kvh, row0;  // first row within the sequence's R
   int q0, q_len, kv;   // first token, new tokens, cached tokens of the sequence
   int a, b, n;
+  int first, pieces;   // run of the item's first piece, and its pieces
 };
 
-// Tiles of item i of a sequence.  The walk is 32-bit arithmetic: the host bounds the number of tiles below
+// Tiles of item i of a sequence.  The walk is 32-bit arithmetic: the host bounds the length of all work below
 // 2^31, and the 64-bit divisions cost a decode step more than its loads.
-__device__ __forceinline__ int paged_tiles(int i, int rpi, int g, int q_len, int kv, int causal, int kt) {
+__device__ __forceinline__ int paged_tiles(const PagedParams& p, int i, int q_len, int kv, int kt) {
   int keys = kv;
-  if (causal) {
-    const unsigned last = (min((unsigned)(i + 1) * (unsigned)rpi, (unsigned)q_len * (unsigned)g) - 1u) / (unsigned)g;
-    keys = max(0, kv - q_len + (int)last + 1);
+  if (p.causal) {
+    const unsigned rows = min((unsigned)(i + 1) * (unsigned)p.rpi, (unsigned)q_len * (unsigned)p.g);
+    keys = max(0, kv - q_len + (int)((rows - 1u) / (unsigned)p.g) + 1);
   }
   return max(1, (int)(((unsigned)keys + (unsigned)kt - 1u) / (unsigned)kt));
 }
@@ -77,111 +79,119 @@ __device__ __forceinline__ void paged_lens(const PagedParams& p, int s, int& q0,
     kv = (int)min((long long)kv, most);
   }
 }
-__device__ __forceinline__ int paged_seq_work(const PagedParams& p, int s, int kt) {
-  if (s >= p.pg.seqs) return 0;
-  int q0, q_len, kv;
-  paged_lens(p, s, q0, q_len, kv);
-  const int n = paged_items(q_len, p.g, p.rpi);
-  if (n == 0) return 0;
-  int w = n * p.item_cost;
-  if (!p.causal || n == 1) return w + n * paged_tiles(0, p.rpi, p.g, q_len, kv, p.causal, kt);
-  for (int i = 0; i < n; ++i) w += paged_tiles(i, p.rpi, p.g, q_len, kv, 1, kt);
-  return w;
-}
 
-// A run of tiles, walked item by item by one warp (every lane holds the same state).
+// A run, walked item by item by one warp (every lane holds the same state).  KT keys make a tile; W is its
+// time, HW that of one of an item of at most half_rows rows.
+template <int KT, int W = 1, int HW = 1>
 struct PagedWalk {
-  int left, chunk;  // tiles left in the run; tiles per run (item costs included)
-  int cost;         // of the next item's start, not yet taken off `left`
-  int seq, kvh, item, tile;
+  int begin, end, chunk;  // the run; its length, that of all runs but the last
+  int pos;                // where the next item begins
+  int seq, kvh, item;
   int q0, q_len, kv, items;
 
+  __device__ __forceinline__ static int weight(const PagedParams& p, int i, int q_len) {
+    if constexpr (W == HW) return W;
+    return q_len * p.g - i * p.rpi <= p.half_rows ? HW : W;
+  }
+  __device__ __forceinline__ static int work(const PagedParams& p, int s) {  // of one KV head of sequence s
+    if (s >= p.pg.seqs) return 0;
+    int q0, q_len, kv;
+    paged_lens(p, s, q0, q_len, kv);
+    const int n = paged_items(q_len, p.g, p.rpi);
+    if (n == 0) return 0;
+    int w = n * p.item_cost + weight(p, n - 1, q_len) * paged_tiles(p, n - 1, q_len, kv, KT);
+    if (!p.causal) return w + (n - 1) * W * paged_tiles(p, 0, q_len, kv, KT);
+    for (int i = 0; i < n - 1; ++i) w += W * paged_tiles(p, i, q_len, kv, KT);
+    return w;
+  }
   // Run `run` of `runs`.
-  __device__ __forceinline__ void start(const PagedParams& p, int kt, int run, int runs) {
+  __device__ __forceinline__ void start(const PagedParams& p, int run, int runs) {
     const int lane = (int)lane_id();
-    seq = kvh = item = tile = q0 = q_len = kv = items = cost = 0;  // an empty run is never walked
-    const int w0 = paged_seq_work(p, lane, kt);
+    begin = end = pos = seq = kvh = item = q0 = q_len = kv = items = 0;  // an empty run is never walked
+    const int w0 = work(p, lane);
     int total = w0;
 #pragma unroll 1
-    for (int s = lane + 32; s < p.pg.seqs; s += 32) total += paged_seq_work(p, s, kt);
+    for (int s = lane + 32; s < p.pg.seqs; s += 32) total += work(p, s);
     total = __reduce_add_sync(0xffffffffu, total) * p.Hkv;
-    chunk = max(1, (int)(((unsigned)total + (unsigned)runs - 1u) / (unsigned)runs));
-    int at = (int)min((unsigned)run * (unsigned)chunk, (unsigned)total);
-    left = min(chunk, total - at);
-    if (left <= 0) return;
+    chunk = max(W > HW ? W : HW, (int)(((unsigned)total + (unsigned)runs - 1u) / (unsigned)runs));
+    const int from = (int)min((unsigned)run * (unsigned)chunk, (unsigned)total);
+    if (from >= total) return;
+    int at = from;
 #pragma unroll 1
     for (int s0 = 0; s0 < p.pg.seqs; s0 += 32) {
-      const int per_head = s0 == 0 ? w0 : paged_seq_work(p, s0 + lane, kt);
-      int end = per_head * p.Hkv;  // inclusive prefix sum
+      const int per_head = s0 == 0 ? w0 : work(p, s0 + lane);
+      int sum = per_head * p.Hkv;  // inclusive prefix sum
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, end, o);
-        if (lane >= o) end += v;
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, at < end);
+      const unsigned hit = __ballot_sync(0xffffffffu, at < sum);
       if (hit != 0) {
         const int l = __ffs(hit) - 1;
         const unsigned head_work = (unsigned)__shfl_sync(0xffffffffu, per_head, l);
-        at -= __shfl_sync(0xffffffffu, end, l) - (int)head_work * p.Hkv;
+        at -= __shfl_sync(0xffffffffu, sum, l) - (int)head_work * p.Hkv;
         seq = s0 + l;
         enter(p);
         kvh = (int)((unsigned)at / head_work);
         at -= kvh * (int)head_work;
-        item = 0;
 #pragma unroll 1
-        for (int n; at >= (n = p.item_cost + paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt)); ++item) at -= n;
-        tile = max(0, at - p.item_cost);
-        cost = max(0, p.item_cost - at);
+        for (int n; at >= (n = length(p)); ++item) at -= n;
+        pos = from - at;
+        begin = from;
+        end = min(from + chunk, total);
         return;
       }
-      at -= __shfl_sync(0xffffffffu, end, 31);
+      at -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    left = 0;
   }
   __device__ __forceinline__ void enter(const PagedParams& p) {
     paged_lens(p, seq, q0, q_len, kv);
     items = paged_items(q_len, p.g, p.rpi);
   }
+  __device__ __forceinline__ int length(const PagedParams& p) const {
+    return p.item_cost + weight(p, item, q_len) * paged_tiles(p, item, q_len, kv, KT);
+  }
   // The next piece; false at the end of the run.
-  __device__ __forceinline__ bool next(const PagedParams& p, int kt, PagedItem& x) {
-    left = max(0, left - cost);
-    cost = p.item_cost;
-    if (left == 0) return false;
-    x.seq = seq;
-    x.kvh = kvh;
-    x.row0 = item * p.rpi;
-    x.q0 = q0;
-    x.q_len = q_len;
-    x.kv = kv;
-    x.n = paged_tiles(item, p.rpi, p.g, q_len, kv, p.causal, kt);
-    x.a = tile;
-    x.b = min(x.n, tile + left);
-    left -= x.b - x.a;
-    tile = 0;
-    if (++item >= items) {
-      item = 0;
-      if (++kvh >= p.Hkv) {
-        kvh = 0;
-        if (left > cost) {
+  __device__ __forceinline__ bool next(const PagedParams& p, PagedItem& x) {
 #pragma unroll 1
-          do {
-            ++seq;
-            enter(p);
-          } while (items == 0 && seq + 1 < p.pg.seqs);  // work is left, so a sequence with tokens follows
-        } else {
-          left = 0;
+    while (pos < end) {
+      const int w = weight(p, item, q_len), at = pos + p.item_cost;
+      x.seq = seq;
+      x.kvh = kvh;
+      x.row0 = item * p.rpi;
+      x.q0 = q0;
+      x.q_len = q_len;
+      x.kv = kv;
+      x.n = paged_tiles(p, item, q_len, kv, KT);
+      x.a = begin > at ? (begin - at) / w : 0;
+      x.b = end > at ? min(x.n, (end - at) / w) : 0;
+      x.first = (int)((unsigned)(at + w - 1) / (unsigned)chunk);
+      x.pieces = (int)((unsigned)(at + x.n * w - 1) / (unsigned)chunk) - x.first + 1;
+      pos = at + x.n * w;
+      if (++item >= items) {
+        item = 0;
+        if (++kvh >= p.Hkv) {
+          kvh = 0;
+          if (pos < end) {
+#pragma unroll 1
+            do {
+              ++seq;
+              enter(p);
+            } while (items == 0 && seq + 1 < p.pg.seqs);  // work is left, so a sequence with tokens follows
+          }
         }
       }
+      if (x.a < x.b) return true;
     }
-    return true;
+    return false;
   }
 };
 
 // The split item that begins in a CTA's run, for the join: x = the sequence's first token, y = KV head,
 // z = first row, w = pieces << 16 | rows (0: none begins here).
-__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x, int chunk) {
-  const int pieces = 1 + (int)((unsigned)(x.n - x.b + chunk - 1) / (unsigned)chunk);
-  return make_int4(x.q0, x.kvh, x.row0, pieces << 16 | min(p.rpi, x.q_len * p.g - x.row0));
+__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x) {
+  return make_int4(x.q0, x.kvh, x.row0, x.pieces << 16 | min(p.rpi, x.q_len * p.g - x.row0));
 }
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
 __device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
@@ -198,13 +208,7 @@ struct PagedPieces {
   int first, n;
   __device__ __forceinline__ long long slot(int i) const { return i == 0 ? 2LL * first + 1 : 2LL * (first + i); }
 };
-__device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x, int chunk) {
-  // a piece that continues an item is its run's first, so the item begins x.a tiles before the run
-  if (x.a == 0) return PagedPieces{(int)blockIdx.x, 1 + (int)((unsigned)(x.n - x.b + chunk - 1) / (unsigned)chunk)};
-  const unsigned begin = blockIdx.x * (unsigned)chunk - (unsigned)x.a;
-  const unsigned first = begin / (unsigned)chunk;
-  return PagedPieces{(int)first, (int)((begin + (unsigned)x.n - 1u) / (unsigned)chunk - first) + 1};
-}
+__device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x) { return PagedPieces{x.first, x.pieces}; }
 
 // Pieces finished per split item (by its first run) and part of its rows, a set of counters per launch
 // in flight: the host rotates the sets launch by launch, as it does g_sched's slots, and the last
@@ -285,9 +289,9 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
   const int ty = tid >> 4, tx = tid & 15;
   pdl_launch_dependents();
   pdl_wait();
-  PagedWalk walk;
+  PagedWalk<KT> walk;
   if (warp_id() == 0) {
-    walk.start(p, KT, (int)blockIdx.x, (int)gridDim.x);
+    walk.start(p, (int)blockIdx.x, (int)gridDim.x);
     if (tid == 0) p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   const int group = p.g;
@@ -295,11 +299,11 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
     __syncthreads();
     if (warp_id() == 0) {
       PagedItem x;
-      const bool ok = walk.next(p, KT, x);
+      const bool ok = walk.next(p, x);
       if (tid == 0) {
         more = ok ? 1 : 0;
         item = x;
-        if (ok && x.a == 0 && x.b < x.n) p.heads[blockIdx.x] = paged_head(p, x, walk.chunk);
+        if (ok && x.a == 0 && x.b < x.n) p.heads[blockIdx.x] = paged_head(p, x);
       }
     }
     __syncthreads();

@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vcb = lane >> 4;  // V, transposed on load
   const int cr = lane / CH, cc = lane % CH;                               // copies: key cr + RPL i, chunk cc
 
-  PagedWalk walk;  // every warp holds the same
-  walk.start(p, kDecKt, (int)blockIdx.x, (int)gridDim.x);
+  PagedWalk<kDecKt> walk;  // every warp holds the same
+  walk.start(p, (int)blockIdx.x, (int)gridDim.x);
   auto steps_of = [](const PagedItem& x) {  // steps of a piece, at least one
     const int key0 = x.a * kDecKt;
     return (min(x.b * kDecKt, max(x.kv, key0 + 1)) - key0 + KS - 1) / KS;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
 
   // The copies run ahead of the arithmetic on a walk of their own: the warp's next step is step fs of
   // piece fx, `off` the cache offset of its key (lane % KS), -1 for none.
-  PagedWalk fwalk = walk;
+  PagedWalk<kDecKt> fwalk = walk;
   PagedItem fx;
   int fs = 0, fn = 0;
   bool fon = true;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   auto seek = [&]() {
 #pragma unroll 1
     while (fon && fs >= fn) {
-      fon = fwalk.next(p, kDecKt, fx);
+      fon = fwalk.next(p, fx);
       if (fon) {
         fs = warp;
         fn = steps_of(fx);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   uint32_t merges = 0;
   bool primed = false;
 #pragma unroll 1
-  while (walk.next(p, kDecKt, x)) {
+  while (walk.next(p, x)) {
     load_q(x);  // used after the first keys have come
     if (!primed) {
       primed = true;
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
     const int rows = min(p.rpi, x.q_len * p.g - x.row0);
     const bool whole = x.a == 0 && x.b == x.n;
     const long long slot = paged_slot(x);
-    const PagedPieces pc = paged_pieces(x, walk.chunk);
+    const PagedPieces pc = paged_pieces(x);
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += 8) {  // rows r0 .. r0 + 7; the upper eight move down for their turn
       if (r0 == 8) {

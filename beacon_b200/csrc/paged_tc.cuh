@@ -61,9 +61,9 @@ enum : unsigned int {
 };
 
 constexpr int kPtcItems = 4;  // items published ahead
-// An item's start and end against a key tile (16 sequences of 1-512 new tokens after 100-7500: cost 0 138 us,
-// 1 119 us, 2 112 us, 4 110 us; 64 sequences of 1-40 new tokens: 169, 143, 135, 130 us).
-constexpr int kPtcItemCost = 4;
+// Time of a key tile, of one of a dual item, and of an item's start and end (clock counts of every CTA of a
+// launch over 16 sequences of 1-512 new tokens, fitted: 3390, 2330 and 7550 cycles).
+constexpr int kPtcTile = 3, kPtcDualTile = 2, kPtcItemCost = 7;
 struct PtcItem {
   int valid;
   int seq, kvh, tok0;  // sequence; KV head; first token row of the item in q
@@ -243,15 +243,15 @@ __global__ void __launch_bounds__(384, 1)
         pdl_launch_dependents();
         p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
       }
-      PagedWalk walk;
-      walk.start(p, 128, (int)blockIdx.x, (int)gridDim.x);
+      PagedWalk<128, kPtcTile, kPtcDualTile> walk;
+      walk.start(p, (int)blockIdx.x, (int)gridDim.x);
       const int nbox = 128 / tp.box;
       const uint32_t q_tile_bytes = (uint32_t)(tp.tpt * p.g) * 128u * (D / 64);
       uint32_t tk = 0, kissued = 0, kpar = 0, qissued = 0, qpar = 0;
       bool ok = true;
       for (int ci = 0; ok; ++ci) {
         PagedItem w{};
-        const bool more = walk.next(p, 128, w);
+        const bool more = walk.next(p, w);
         PtcItem x{};
         x.valid = more ? 1 : 0;
         if (more) {
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(384, 1)
           x.slot = (w.a == 0 && w.b == w.n) ? -1 : paged_slot(w);
           x.a = w.a;
           x.b = w.b;
-          x.pieces = paged_pieces(w, walk.chunk);
+          x.pieces = paged_pieces(w);
           x.dual = x.ntok <= tp.tpt ? 1 : 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(384, 1)
         if (lane == 0) {
           items[is] = x;
           mbar_arrive(&item_full[is]);
-          if (more && w.a == 0 && w.b < w.n && x.pieces.n > 2) p.heads[blockIdx.x] = paged_head(p, w, walk.chunk);
+          if (more && w.a == 0 && w.b < w.n && x.pieces.n > 2) p.heads[blockIdx.x] = paged_head(p, w);
         }
         if (!more) break;
         int page = (int)lane < nbox ? ptc_page(p.pg, w.seq, x.a * 128 + (int)lane * tp.box, w.kv) : 0;
