@@ -269,6 +269,10 @@ constexpr size_t paged_simt_smem() {
          sizeof(long long) * 2 * kPagedSimtKt;
 }
 
+// Exact form: products and sums in fp32 FFMA, 64 rows x 64 keys per step, 4 x 4 scores per thread, keys and
+// values copied a tile ahead.  Bound: FFMA issue for long work, the chain of a tile's two products for
+// short (8 sequences of 33-1500 keys, 1-40 new tokens, 8 / 4 heads of 64: 27 us).  Also takes bf16 calls that
+// neither other kernel can: head_dim 16 and 32, and rows that are not 16-byte aligned.
 // ASYNC: T is float and the caches' rows are 16-byte aligned.
 template <typename T, int D, bool ASYNC>
 __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q, const T* __restrict__ kc,
@@ -469,7 +473,8 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
 // Joins the split items that p.heads lists: their blocks of 32 rows x 16 columns are dealt out to the
 // grid's warps, a row per lane.  The item that begins in run c has its first piece in slot 2c + 1 and
 // the others in slots 2(c + 1), 2(c + 2), .. in order.  With M = max m:
-// out = sum 2^(m - M) O / sum 2^(m - M) l.
+// out = sum 2^(m - M) O / sum 2^(m - M) l.  Bound: latency (its pieces are read side by side): 5.4 us alone
+// after 2048 new tokens over 32768 keys; launched ahead, it starts as the attention kernel ends.
 constexpr int kPagedMostRuns = 320;  // of any attention kernel that leaves its joins to this one
 template <typename T>
 __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int runs) {

@@ -24,6 +24,11 @@
 // of an item in two pieces are joined by the warp that finishes the second one; k_paged_join joins
 // those of items in more (one warp that reads 16 pieces took 45 us, the whole device a few).
 //
+// Bound: the softmax warps beside the tensor core.  2048 new tokens after 30720, 64/8 heads of 128: 1.70 ms =
+// 1.25 PFLOP/s, tensor pipe active 70% of the cycles.  A 256-row step of 128 keys takes ~3.0k cycles, of them
+// ~1.75k in softmax and ~1.2k waiting for the S that was issued behind the other tile's PV.  Short items pay
+// ~7.5k cycles for their start and end (rows stored from registers, first softmax of both tiles at once).
+//
 // TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
 #pragma once
 

@@ -298,6 +298,11 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd_any(T* __restrict__ dq
 // gains stay in registers and a token's cosines and sines are loaded once per batch.  Each lane
 // copies its chunks of the next kRopeStages - 1 tokens to shared memory ahead (cp.async; only the
 // lane itself reads them, so nothing synchronises): the bytes in flight do not cost registers.
+// Two stages, two CTAs of eight warps per SM: a third CTA spilled, and equal runs of one kind of head per
+// warp scattered the streams (forward 72 -> 86 us).
+// Measured: forward, 8192 tokens of 32 + 32 + 32 heads of 128, bf16: 71.6 us, 403 MB, 5.6 TB/s; a copy with
+// this access pattern alone 69 us.  Prompts of 10k tokens, 64 / 8 heads, into pages of 64: 81.5 us, 4.9 TB/s.
+// What is left: issue slots (41-53% used) and 16 warps per SM to cover the rest with.
 // ---------------------------------------------------------------------------
 constexpr int kRopeStages = 2;
 
@@ -631,7 +636,8 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_vec(T* __restrict__ q, 
 }
 
 // Backward; part as in k_qk_norm_rope_bwd_any.  A warp keeps the partial sums of its kind's gain
-// gradient for its 16 columns in registers over all its tokens.
+// gradient for its 16 columns in registers over all its tokens.  32768 tokens, 32 / 8 heads of 128, bf16:
+// 216 us with both gain sums, 1.14 GB, 5.3 TB/s; a copy with this access pattern alone 185 us.
 template <typename T, int D, int U>
 __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__ dqkv, float* __restrict__ part,
                                                                  const T* __restrict__ dq, const T* __restrict__ dk,

@@ -23,7 +23,8 @@
  *    (workspace = NULL) share that one buffer: give each stream its own workspace
  *    when such calls may overlap.  The persistent kernels (attention forward, dK/dV, dQ)
  *    take their work items from one of 64 counter slots per device, rotating
- *    launch by launch and reset by each launch's last CTA: up to 64 such
+ *    launch by launch and reset by each launch's last CTA; paged attention counts the
+ *    finished pieces of split work in one of the same slots: up to 64 such
  *    launches may be in flight on one device at once.
  *  - Return value: a beacon_status that maps 1:1 onto beacon-cuda's LaunchError
  *    variants (crates/beacon-cuda/src/error.rs:4-13); 0 is Ok.  The message of
@@ -102,7 +103,7 @@ int beacon_diag_wait_timeout(uint64_t limit_ns, unsigned int* out, void* stream)
 int beacon_diag_exp2_poly(float* out, const float* in, int64_t n, void* stream);
 
 /* Device timing of the tensor-core kernels (k_gemm_bf16_tc, k_attn_fwd_tc,
- * k_attn_bwd_dkdv, k_attn_bwd_dq): while enabled, each launch is bracketed by CUDA events on its
+ * k_attn_bwd_dkdv, k_attn_bwd_dq, k_paged_attn_tc, k_paged_attn_dec): while enabled, each launch is bracketed by CUDA events on its
  * own stream.  beacon_profile_read(name, ...) waits for those events and returns the
  * accumulated milliseconds and launch count for `name`; name == NULL resets.
  * No reference counterpart (the reference bench is a stub,
