@@ -234,6 +234,23 @@ __device__ __forceinline__ bool paged_last_piece(int slot, const PagedPieces& pc
   return last != 0u;
 }
 
+// One warp, before its part of a piece is written: whether that part of every other piece has been.  If so
+// this piece's rows need not be written.
+__device__ __forceinline__ bool paged_others_done(int slot, const PagedPieces& pc, int part) {
+  __syncwarp();
+  unsigned int all = 0u;
+  if (lane_id() == 0) {
+    unsigned int* done = &g_paged_done[slot][pc.first][part];
+    unsigned int n;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(done) : "memory");
+    all = n == (unsigned int)pc.n - 1u ? 1u : 0u;
+    if (all) *reinterpret_cast<volatile unsigned int*>(done) = 0u;  // for the launch that takes the set next
+  }
+  all = __shfl_sync(0xffffffffu, all, 0);
+  __syncwarp();
+  return all != 0u;
+}
+
 // Keys that row r (of R) of a piece sees.
 __device__ __forceinline__ int paged_limit(const PagedParams& p, const PagedItem& x, int r) {
   return p.causal ? max(0, x.kv - x.q_len + r / p.g + 1) : x.kv;

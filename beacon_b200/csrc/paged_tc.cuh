@@ -666,17 +666,22 @@ __global__ void __launch_bounds__(384, 1)
         // statistics of the row; B keeps its own copy of a dual item's, in rows that the item does not have
         const int ml_row = row + (x.dual ? t * tp.tpt * p.g : 0);
         const long long own = (long long)x.slot * p.rpi + ml_row;
-        if (has) {
+        // mostly the other piece, the first of its run, was written long ago
+        bool last = x.pieces.n == 2 && paged_others_done(p.sched_slot, x.pieces, (int)warp - 4);
+        if (!last) {
+          if (has) {
 #pragma unroll 1
-          for (int c = c0; c < c1; ++c) {
-            uint32_t u[32];
-            load_o(c, u);
-            if (row_ok) store_part(paged_part(p, x.slot, 8 * c, row), u);
+            for (int c = c0; c < c1; ++c) {
+              uint32_t u[32];
+              load_o(c, u);
+              if (row_ok) store_part(paged_part(p, x.slot, 8 * c, row), u);
+            }
           }
+          // without a key tile here: m = -inf, and its O, not written, is not read
+          if (row_ok) p.part_ml[own] = make_float2(m_used, l);
+          last = x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4);
         }
-        // without a key tile here: m = -inf, and its O, not written, is not read
-        if (row_ok) p.part_ml[own] = make_float2(m_used, l);
-        if (x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4)) {
+        if (last) {
           const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second
           const long long that = x.pieces.slot(1 - mine);
           const float2 ml = row_ok ? __ldcg(&p.part_ml[that * p.rpi + ml_row]) : make_float2(-INFINITY, 0.0f);
