@@ -2,7 +2,8 @@
 // page size; definitions and work distribution in paged.cuh.
 //
 // Bound: HBM (each cached key and value is used by the group's rows only, g FLOP per byte).  A 128-row
-// tcgen05 tile would be a few rows full and its chain of S, softmax and PV is longer.  Here a CTA's eight warps take the 16- or 32-key steps of its run in turn, rows as one 16-row
+// tcgen05 tile would be a few rows full and its chain of S, softmax and PV is longer.  Here a CTA's
+// eight warps take the 16- or 32-key steps of its run in turn, rows as one 16-row
 // m16n8k16 tile each, and every warp copies its next steps to shared memory ahead (cp.async,
 // kDecStages deep, 192 KB per SM), across item boundaries too.  At an item's end the warps' rows
 // meet in shared memory, row r merged by warp r % 8 while the others go on; of a split item the warp

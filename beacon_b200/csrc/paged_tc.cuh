@@ -12,7 +12,7 @@
 //   warp 0      producer (whole warp): the run's items (published in a ring), Q tiles, K ring
 //   warp 2      producer of the V ring.  One producer of both let K(j+2) wait for the V stage that PV(j-1)
 //               frees, so that a tile's S came late: 64 sequences of 500-8192 keys, 8 new tokens each,
-//               32/8 heads of 128: 247 us with one, 153 us with two.
+//               32/8 heads of 128: 247 us with one, 153 us with two (144 now).
 //   warp 1      TMEM allocator, MMA issuer:  S_A S_B | O_A += P_A V, S_A', O_B += P_B V, S_B' | ...
 //   warps 4-7   softmax of tile A, warps 8-11 of tile B: one row per thread, fp32 statistics, P (bf16)
 //               back into the S region of TMEM, O rescaled there when the maximum grows by over 2^8.
@@ -27,7 +27,9 @@
 // Bound: the softmax warps beside the tensor core.  2048 new tokens after 30720, 64/8 heads of 128: 1.70 ms =
 // 1.25 PFLOP/s, tensor pipe active 70% of the cycles.  A 256-row step of 128 keys takes ~3.0k cycles, of them
 // ~1.75k in softmax and ~1.2k waiting for the S that was issued behind the other tile's PV.  Short items pay
-// ~7.5k cycles for their start and end (rows stored from registers, first softmax of both tiles at once).
+// ~7.5k cycles for their start and end (rows stored from registers, first softmax of both tiles at once):
+// 16 sequences of 1-512 new tokens after 100-7500, 32/8 heads, 103 us against 45 us of FLOPs.  Their code is
+// fetched anew at each item's end: unrolled by chunk it was slower (106 us).
 //
 // TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
 #pragma once
@@ -712,7 +714,8 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (c + 1 < c1) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = read ? __ldcg(src + (long long)(8 * (c + 1 - c0) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int e = 0; e < 8; ++e)
+                v[e] = read ? __ldcg(src + (long long)(8 * (c + 1 - c0) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             if (row_ok) store_o(c, u, inv, none);
           }
