@@ -133,6 +133,21 @@ def test_long_context_split_over_the_device_repeats_bit_for_bit(dt):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_full_and_short_items_split_in_two_repeat_bit_for_bit(D, causal):
+    """Items of 256 rows and of at most 128 take different times per key tile; most of these fall into two
+    runs, either of which may end last."""
+    import torch
+    c = Case([130, 60, 3, 200, 64, 20, 128, 65], [1900, 1100, 1501, 1280, 1663, 1, 1409, 1153], 16, 8, D, 16, "bf16",
+             seed=D)
+    first = c.run(max_q=200, causal=causal)
+    c.check(*first, causal=causal)
+    for _ in range(5):
+        again = c.run(max_q=200, causal=causal)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_strided_pool_strided_queries_and_unowned_rows(dt):
     """Keys and values interleaved in one pool of another layout ([pages, page, 2, heads, D]), queries as a
