@@ -212,7 +212,7 @@ __device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x) { return
 
 // Pieces finished per split item (by its first run) and part of its rows, a set of counters per launch
 // in flight: the host rotates the sets launch by launch, as it does g_sched's slots, and the last
-// piece resets its counter.
+// piece resets its counter.  After a launch that gave up a wait, beacon_device_status resets them all.
 constexpr int kPagedMaxRuns = 160, kPagedParts = 16;
 __device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns][kPagedParts];
 
