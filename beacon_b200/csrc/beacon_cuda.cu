@@ -651,10 +651,6 @@ extern "C" int beacon_device_status(int device, unsigned int out[3]) {
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(w, g_beacon_status, sizeof(w));
   const unsigned int zero[4] = {0, 0, 0, 0};
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_beacon_status, zero, sizeof(zero));
-  // a paged attention that gave up a wait leaves pieces uncounted, and its set of counters is used again
-  void* done = nullptr;
-  if (e == cudaSuccess && w[0] == kFaultWaitTimeout) e = cudaGetSymbolAddress(&done, g_paged_done);
-  if (e == cudaSuccess && done != nullptr) e = cudaMemset(done, 0, sizeof(g_paged_done));
   cudaSetDevice(prev);
   if (e != cudaSuccess) return fail(BEACON_ERR_CUDA, "device status: %s", cudaGetErrorString(e));
   if (out) {

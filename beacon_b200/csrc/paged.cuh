@@ -33,8 +33,8 @@ struct PagedParams {
   long long tokens;
   void* out;                 // [tokens, Hq, D]
   float* lse;                // [tokens, Hq] or null
-  int sched_slot;            // row of g_paged_done
   int4* heads;               // [gridDim.x] the split item that begins in this CTA's run (paged_head)
+  unsigned int* done;        // [gridDim.x, kPagedParts] finished pieces (paged_last_piece)
   float* part_o;             // [slots, D / 4, rpi, 4] (paged_part)
   float2* part_ml;           // [2 * gridDim.x, rpi] (running maximum, in log2 units; sum)
 };
@@ -210,24 +210,30 @@ struct PagedPieces {
 };
 __device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x) { return PagedPieces{x.first, x.pieces}; }
 
-// Pieces finished per split item (by its first run) and part of its rows, a set of counters per launch
-// in flight: the host rotates the sets launch by launch, as it does g_sched's slots, and the last
-// piece resets its counter.  After a launch that gave up a wait, beacon_device_status resets them all.
+// Pieces finished per split item (by its first run) and part of its rows.  The counters lie in the call's
+// workspace and k_paged_clear, launched ahead on the stream, zeroes them for every execution of the call,
+// replays of a captured one included: whatever the workspace held before, and whatever runs beside the
+// call with a workspace of its own, no count of another launch is ever seen.
 constexpr int kPagedMaxRuns = 160, kPagedParts = 16;
-__device__ unsigned int g_paged_done[kSchedSlots][kPagedMaxRuns][kPagedParts];
+__global__ void __launch_bounds__(256) k_paged_clear(uint4* __restrict__ done, int n) {
+  pdl_launch_dependents();
+  pdl_wait();
+  for (int i = (int)(blockIdx.x * 256 + threadIdx.x); i < n; i += (int)gridDim.x * 256) done[i] = make_uint4(0u, 0u, 0u, 0u);
+}
 
 // One warp, after its part of a piece has been written: whether that part of every piece now has been.  One
 // lane's release-acquire add stands for the warp, ordered with the others' accesses by the warp
 // barriers around it (a fence in every lane and a relaxed add took twice as long).
-__device__ __forceinline__ bool paged_last_piece(int slot, const PagedPieces& pc, int part) {
+__device__ __forceinline__ bool paged_last_piece(const PagedParams& p, const PagedPieces& pc, int part) {
   __syncwarp();
   unsigned int last = 0u;
   if (lane_id() == 0) {
-    unsigned int* done = &g_paged_done[slot][pc.first][part];
     unsigned int before;
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(done) : "memory");
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                 : "=r"(before)
+                 : "l"(p.done + pc.first * kPagedParts + part)
+                 : "memory");
     last = before == (unsigned int)pc.n - 1u ? 1u : 0u;
-    if (last) *reinterpret_cast<volatile unsigned int*>(done) = 0u;  // for the launch that takes the set next
   }
   last = __shfl_sync(0xffffffffu, last, 0);
   __syncwarp();
@@ -236,15 +242,13 @@ __device__ __forceinline__ bool paged_last_piece(int slot, const PagedPieces& pc
 
 // One warp, before its part of a piece is written: whether that part of every other piece has been.  If so
 // this piece's rows need not be written.
-__device__ __forceinline__ bool paged_others_done(int slot, const PagedPieces& pc, int part) {
+__device__ __forceinline__ bool paged_others_done(const PagedParams& p, const PagedPieces& pc, int part) {
   __syncwarp();
   unsigned int all = 0u;
   if (lane_id() == 0) {
-    unsigned int* done = &g_paged_done[slot][pc.first][part];
     unsigned int n;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(done) : "memory");
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(p.done + pc.first * kPagedParts + part) : "memory");
     all = n == (unsigned int)pc.n - 1u ? 1u : 0u;
-    if (all) *reinterpret_cast<volatile unsigned int*>(done) = 0u;  // for the launch that takes the set next
   }
   all = __shfl_sync(0xffffffffu, all, 0);
   __syncwarp();

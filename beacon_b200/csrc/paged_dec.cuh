@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
 #pragma unroll
       for (int e = 0; e < CPL; ++e) po[e] = ot[e];
       if (lane == 0) p.part_ml[slot * p.rpi + r] = make_float2(mx, lt);
-      if (!paged_last_piece(p.sched_slot, pc, r)) continue;
+      if (!paged_last_piece(p, pc, r)) continue;
       // lane i weighs piece i (of 32 at a time); the pieces' rows then load side by side
       mx = -INFINITY;
       for (int i = lane; i < pc.n; i += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);

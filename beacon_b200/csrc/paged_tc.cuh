@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(384, 1)
         const int ml_row = row + (x.dual ? t * tp.tpt * p.g : 0);
         const long long own = (long long)x.slot * p.rpi + ml_row;
         // mostly the other piece, the first of its run, was written long ago
-        bool last = x.pieces.n == 2 && paged_others_done(p.sched_slot, x.pieces, (int)warp - 4);
+        bool last = x.pieces.n == 2 && paged_others_done(p, x.pieces, (int)warp - 4);
         if (!last) {
           if (has) {
 #pragma unroll 1
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(384, 1)
           }
           // without a key tile here: m = -inf, and its O, not written, is not read
           if (row_ok) p.part_ml[own] = make_float2(m_used, l);
-          last = x.pieces.n == 2 && paged_last_piece(p.sched_slot, x.pieces, (int)warp - 4);
+          last = x.pieces.n == 2 && paged_last_piece(p, x.pieces, (int)warp - 4);
         }
         if (last) {
           const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second

@@ -23,9 +23,11 @@
  *    (workspace = NULL) share that one buffer: give each stream its own workspace
  *    when such calls may overlap.  The persistent kernels (attention forward, dK/dV, dQ)
  *    take their work items from one of 64 counter slots per device, rotating
- *    launch by launch and reset by each launch's last CTA; paged attention counts the
- *    finished pieces of split work in one of the same slots: up to 64 such
- *    launches may be in flight on one device at once.
+ *    launch by launch and reset by each launch's last CTA: up to 64 such
+ *    launches may be in flight on one device at once.  A captured launch keeps the
+ *    slot of its capture: replay it only while none of these kernels that another
+ *    stream launched is in flight.  Paged attention counts in its workspace
+ *    and has no such limit.
  *  - Return value: a beacon_status that maps 1:1 onto beacon-cuda's LaunchError
  *    variants (crates/beacon-cuda/src/error.rs:4-13); 0 is Ok.  The message of
  *    the last error on the calling thread is available from beacon_last_error().
