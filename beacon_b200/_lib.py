@@ -188,7 +188,8 @@ def front():
         spec.loader.exec_module(mod)
         mod.bind(*(ctypes.cast(getattr(lib(), n), _vp).value for n in (
             "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd", "beacon_qk_norm_rope_append",
-            "beacon_paged_attention_fwd")))
+            "beacon_paged_attention_fwd", "beacon_qk_norm_rope_bwd_workspace_size",
+            "beacon_paged_attention_workspace_size")))
         _front = mod
     return _front
 

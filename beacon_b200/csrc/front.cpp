@@ -21,6 +21,8 @@ decltype(&beacon_qk_norm_rope_fwd) g_fwd = nullptr;
 decltype(&beacon_qk_norm_rope_bwd) g_bwd = nullptr;
 decltype(&beacon_qk_norm_rope_append) g_append = nullptr;
 decltype(&beacon_paged_attention_fwd) g_attn = nullptr;
+decltype(&beacon_qk_norm_rope_bwd_workspace_size) g_bwd_ws = nullptr;
+decltype(&beacon_paged_attention_workspace_size) g_attn_ws = nullptr;
 
 using at::Tensor;
 
@@ -105,6 +107,11 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 Tensor make(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options()); }
 
+// A call's scratch from the caching allocator: ordered on the call's stream, and kept by a graph that captures it.
+Tensor scratch(size_t bytes, const Tensor& like) {
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
 PyObject* status(int rc) { return PyLong_FromLong(rc); }
 
 // A call's body: C++ exceptions (an allocation that fails) become Python ones.
@@ -167,10 +174,12 @@ PyObject* front_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !rope(r, width, D))
       Py_RETURN_NONE;
     Tensor dx = make({B * S, width}, *dq), dqg = make({D}, *dq), dkg = make({D}, *dq);
+    const size_t need = g_bwd_ws(D);
+    Tensor ws = scratch(need, *dq);
     const int rc = g_bwd(dx.data_ptr(), width, dqg.data_ptr(), dkg.data_ptr(), dq->data_ptr(), dk->data_ptr(),
                          dv->data_ptr(), r.qkv->data_ptr(), r.ld, ptr(r.q_gain), ptr(r.k_gain),
                          (const float*)ptr(r.table), r.rows, (const int32_t*)ptr(r.positions), B, S, H, K, D, r.rot,
-                         r.interleaved, r.eps, dtype_code(dt), nullptr, 0, stream());
+                         r.interleaved, r.eps, dtype_code(dt), ws.data_ptr(), need, stream());
     return rc != BEACON_OK ? status(rc) : pack3(dx, dqg, dkg);
   });
 }
@@ -216,23 +225,25 @@ PyObject* front_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     const int64_t T = q->size(0), H = q->size(1);
     Tensor out = make({T, H, g.dim}, *q), lse = at::empty({T, H}, q->options().dtype(at::kFloat));
+    const size_t need = g_attn_ws(g.dim, dtype_code(q->scalar_type()));
+    Tensor ws = scratch(need, *q);
     const int rc = g_attn(out.data_ptr(), (float*)lse.data_ptr(), q->data_ptr(),
                           T > 1 ? q->stride(0) : std::max(q->stride(0), H * g.dim), g.k->data_ptr(), g.v->data_ptr(),
                           (const int32_t*)ptr(g.cu_q), (const int32_t*)ptr(g.kv_lens), (const int32_t*)ptr(g.table), T,
                           g.seqs, max_q, g.width, g.stride, g.pages, g.page, g.k->stride(0), g.k->stride(1),
                           token_stride(g), H, g.heads, g.dim, PyObject_IsTrue(a[7]), dtype_code(q->scalar_type()),
-                          nullptr, 0, stream());
+                          ws.data_ptr(), need, stream());
     return rc != BEACON_OK ? status(rc) : Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
   });
 }
 
-// bind(fwd, bwd, append, attention): addresses of the C entry points
+// bind(fwd, bwd, append, attention, bwd_workspace_size, attention_workspace_size): addresses of the C entry points
 PyObject* front_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* p[4];
-  for (int i = 0; i < 4; ++i) {
-    p[i] = n == 4 ? PyLong_AsVoidPtr(a[i]) : nullptr;
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
+    p[i] = n == 6 ? PyLong_AsVoidPtr(a[i]) : nullptr;
     if (p[i] == nullptr) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: four addresses");
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: six addresses");
       return nullptr;
     }
   }
@@ -240,6 +251,8 @@ PyObject* front_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_bwd = reinterpret_cast<decltype(g_bwd)>(p[1]);
   g_append = reinterpret_cast<decltype(g_append)>(p[2]);
   g_attn = reinterpret_cast<decltype(g_attn)>(p[3]);
+  g_bwd_ws = reinterpret_cast<decltype(g_bwd_ws)>(p[4]);
+  g_attn_ws = reinterpret_cast<decltype(g_attn_ws)>(p[5]);
   Py_RETURN_NONE;
 }
 

@@ -217,6 +217,14 @@ def _refuse(what, *tests):
     raise InvalidLaunchConfig(f"{what}: operands do not fit")
 
 
+def _scratch(workspace, need, device):
+    """(workspace, its bytes); one of `need` bytes from torch's allocator, which orders it on the stream and keeps
+    it for a graph that captures the call, where the caller gave none."""
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, workspace.numel() * workspace.element_size()
+
+
 def _dense_i32(t, n):
     return t.dtype is torch.int32 and t.is_cuda and t.numel() == n and t.is_contiguous()
 
@@ -324,11 +332,11 @@ def qk_norm_rope_bwd(dq, dk, dv, qkv, q_gain, k_gain, table, positions=None, int
     dqkv = torch.empty((B * S, width), dtype=dq.dtype, device=dq.device)
     dqg = None if q_gain is None else torch.empty_like(q_gain)
     dkg = None if k_gain is None else torch.empty_like(k_gain)
-    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    workspace, wsb = _scratch(workspace, _lib.lib().beacon_qk_norm_rope_bwd_workspace_size(D), dq.device)
     check(_lib.lib().beacon_qk_norm_rope_bwd(
         dqkv.data_ptr(), width, _p(dqg), _p(dkg), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qkv.data_ptr(), ld,
-        _p(q_gain), _p(k_gain), _p(table), rows, _p(positions), B, S, H, Hkv, D, rot, int(interleaved), eps, dt, ws, wsb,
-        _stream()))
+        _p(q_gain), _p(k_gain), _p(table), rows, _p(positions), B, S, H, Hkv, D, rot, int(interleaved), eps, dt,
+        _p(workspace), wsb, _stream()))
     return dqkv, dqg, dkg
 
 
@@ -394,11 +402,11 @@ def paged_attention(q, k_cache, v_cache, page_table, cu_q, kv_lens, max_q=0, cau
         lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
     elif lse.shape != (T, H) or lse.dtype is not torch.float32 or not lse.is_contiguous() or not lse.is_cuda:
         raise InvalidLaunchConfig(f"paged_attention: lse must be a contiguous float32 {(T, H)}")
-    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    workspace, wsb = _scratch(workspace, paged_attention_workspace_bytes(D, dtype), q.device)
     check(_lib.lib().beacon_paged_attention_fwd(
         out.data_ptr(), lse.data_ptr(), q.data_ptr(), s0 if T > 1 else max(s0, H * D), k_cache.data_ptr(),
         v_cache.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(), T, seqs, int(max_q or 0), *paging,
-        H, Hkv, D, int(causal), code, ws, wsb, _stream()))
+        H, Hkv, D, int(causal), code, _p(workspace), wsb, _stream()))
     return out, lse
 
 
@@ -579,12 +587,12 @@ def llama_block_paged_fwd(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_do
     rows, rot = (0, 0) if table is None else table.shape
     if out is None:
         out = torch.empty_like(x)
-    ws, wsb = (None, 0) if workspace is None else (_p(workspace), workspace.numel() * workspace.element_size())
+    workspace, wsb = _scratch(workspace, llama_block_paged_workspace_bytes(T, dm, heads, Hkv, D, w_gate.shape[1]), x.device)
     check(_lib.lib().beacon_llama_block_paged_fwd(
         _p(out), _p(x), _p(attn_norm), _p(w_qkv), _p(q_gain), _p(k_gain), _p(w_o), _p(ffn_norm), _p(w_gate), _p(w_up),
         _p(w_down), _p(table), rows, rot, int(interleaved), _p(k_cache), _p(v_cache), _p(cu_q), _p(kv_lens),
-        _p(page_table), T, seqs, int(max_q or 0), *paging, dm, heads, Hkv, D, w_gate.shape[1], eps, dt, ws, wsb,
-        _stream()))
+        _p(page_table), T, seqs, int(max_q or 0), *paging, dm, heads, Hkv, D, w_gate.shape[1], eps, dt,
+        _p(workspace), wsb, _stream()))
     return out
 
 

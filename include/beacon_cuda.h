@@ -363,7 +363,8 @@ int beacon_qk_norm_rope_fwd(void* q, void* k, void* v, const void* qkv, int64_t 
  *   e = g dz, dx = e / r - x sum(e x) / (head_dim r^3)   (dx = dz without a gain).
  * dqkv rows lie dqkv_stride elements apart; dv NULL leaves their value columns as they are.
  * dq_gain, dk_gain [head_dim] may be NULL; their sums are kept in float32 and added in a fixed order
- * (results do not depend on timing).  Workspace as for attention, needed only for gain gradients. */
+ * (results do not depend on timing).  Workspace of beacon_qk_norm_rope_bwd_workspace_size bytes, needed only
+ * for gain gradients, or NULL for the library's; a captured call needs its own (below). */
 int beacon_qk_norm_rope_bwd(void* dqkv, int64_t dqkv_stride, void* dq_gain, void* dk_gain, const void* dq,
                             const void* dk, const void* dv, const void* qkv, int64_t qkv_stride,
                             const void* q_gain, const void* k_gain, const float* table, int64_t table_positions,
@@ -378,7 +379,9 @@ size_t beacon_qk_norm_rope_bwd_workspace_size(int64_t head_dim);
  * token-major tensors and kv_lens[s] cached tokens, the new ones included and last; its token j
  * sits in page page_table[s * table_stride + j / page_size] (max_pages entries per row; entries past the
  * last used page are not read).  cu_q, kv_lens and page_table are int32 in device memory and are read on
- * the stream: no host copy, so the calls can be captured.  A page index outside the cache is not
+ * the stream: no host copy, so the calls can be captured.  A captured call needs a workspace of its own, which
+ * lives as long as its graph: the library's buffer is freed when a later call needs a larger one, so NULL
+ * is refused with InvalidLaunchConfig on a stream that is being captured.  A page index outside the cache is not
  * followed (its tokens are not written, its keys and values read as zeros), and lengths that reach
  * past the tensors are cut; both record fault code 3.  Token rows that no sequence owns are ignored.
  *
@@ -402,7 +405,7 @@ int beacon_qk_norm_rope_append(void* q, void* k_cache, void* v_cache, const void
  * beyond kv_lens never reach a result, NaN included.  max_q: the largest number of new tokens of a
  * sequence if known, else 0; it only chooses between kernels.  head_dim 16, 32, 64 or 128; bf16 or f32
  * (exact fp32 products).  Workspace of beacon_paged_attention_workspace_size bytes, 32-byte aligned
- * (partial rows of work split along the keys), or NULL for the library's. */
+ * (partial rows of work split along the keys; it may hold anything), or NULL for the library's. */
 int beacon_paged_attention_fwd(void* out, float* lse, const void* q, int64_t q_stride, const void* k_cache,
                                const void* v_cache, const int32_t* cu_q, const int32_t* kv_lens,
                                const int32_t* page_table, int64_t tokens, int64_t seqs, int64_t max_q,
@@ -417,8 +420,8 @@ size_t beacon_paged_attention_workspace_size(int64_t head_dim, int dtype);
  * come.  Per-head norms (q_gain, k_gain [head_dim], NULL: none) and the rotation (rope_table NULL with
  * rot_dim 0: none) act on queries and keys before the new keys and values enter the pages; attention is
  * causal over the whole cache.  bf16; the other conditions are beacon_llama_block_fwd's and
- * beacon_paged_attention_fwd's.  Scratch: beacon_llama_block_paged_workspace_size bytes or the library's.
- * Nothing is read back, so a step can be captured.  Rows of out for tokens that no sequence owns are
+ * beacon_paged_attention_fwd's.  Scratch: beacon_llama_block_paged_workspace_size bytes, 32-byte aligned, or NULL
+ * for the library's.  Nothing is read back, so a step can be captured, with a workspace of its own.  Rows of out for tokens that no sequence owns are
  * undefined. */
 int beacon_llama_block_paged_fwd(void* out, const void* x, const void* attn_norm, const void* w_qkv,
                                  const void* q_gain, const void* k_gain, const void* w_o, const void* ffn_norm,
