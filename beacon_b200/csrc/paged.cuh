@@ -4,6 +4,9 @@
 // Sequence s brings q_len = cu_q[s+1] - cu_q[s] new tokens and kv = kv_lens[s] cached ones, the new
 // ones last.  New token i sits at p = kv - q_len + i and sees keys j <= p (causal) or j < kv:
 //   out = softmax(q k^T / sqrt(D)) v, lse = log sum exp; no key visible: out = 0, lse = -inf.
+// A row that sees a score of NaN or +inf, or scores of -inf only, has out = NaN and lse = the logarithm of its
+// sum (NaN, +inf, -inf).  All of that is read off the row's maximum, which keeps NaN (max_nan); whether a
+// row sees a key at all is counted, never read off the maximum.
 // For one KV head the rows are (token, query head of the group), token-major: R = q_len * g.
 //
 // Work: an item is `rpi` consecutive rows of one (sequence, KV head); its length is the time of the
@@ -21,6 +24,14 @@
 
 namespace beacon {
 
+// The split item that begins in a CTA's run, for the join.
+struct __align__(16) PagedHead {
+  int q0, kvh, row0, rows;  // the sequence's first token, KV head, first row and rows (0: none begins here)
+  int pieces;
+  int lim;                  // keys that the sequence's first new token sees (causal; may be negative), or all keys
+  int pad[2];
+};
+
 struct PagedParams {
   PagedSeqs pg;
   int Hq, Hkv, D, g;         // g = Hq / Hkv
@@ -33,7 +44,7 @@ struct PagedParams {
   long long tokens;
   void* out;                 // [tokens, Hq, D]
   float* lse;                // [tokens, Hq] or null
-  int4* heads;               // [gridDim.x] the split item that begins in this CTA's run (paged_head)
+  PagedHead* heads;          // [gridDim.x] the split item that begins in this CTA's run
   unsigned int* done;        // [gridDim.x, kPagedParts] finished pieces (paged_last_piece)
   float* part_o;             // [slots, D / 4, rpi, 4] (paged_part)
   float2* part_ml;           // [2 * gridDim.x, rpi] (running maximum, in log2 units; sum)
@@ -188,10 +199,27 @@ struct PagedWalk {
   }
 };
 
-// The split item that begins in a CTA's run, for the join: x = the sequence's first token, y = KV head,
-// z = first row, w = pieces << 16 | rows (0: none begins here).
-__device__ __forceinline__ int4 paged_head(const PagedParams& p, const PagedItem& x) {
-  return make_int4(x.q0, x.kvh, x.row0, x.pieces << 16 | min(p.rpi, x.q_len * p.g - x.row0));
+__device__ __forceinline__ PagedHead paged_head(const PagedParams& p, const PagedItem& x) {
+  return PagedHead{x.q0, x.kvh, x.row0, min(p.rpi, x.q_len * p.g - x.row0), x.pieces, p.causal ? x.kv - x.q_len + 1 : x.kv};
+}
+
+// Maxima that keep NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// What a row's sums are multiplied by, and its lse, from its maximum m (log2 units) and sum l of 2^(s - m).
+__device__ __forceinline__ float paged_inv(float m, float l) {
+  return fabsf(m) < INFINITY ? 1.0f / l : __uint_as_float(0x7fffffffu);
+}
+__device__ __forceinline__ float paged_lse(float m, float log2_l) {
+  return fabsf(m) < INFINITY ? (m + log2_l) * 0.69314718055994531f : m;
 }
 // Workspace slot of a partial piece: a piece that continues an item is the run's first.
 __device__ __forceinline__ int paged_slot(const PagedItem& x) { return 2 * (int)blockIdx.x + (x.a > 0 ? 0 : 1); }
@@ -317,7 +345,7 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
   PagedWalk<KT> walk;
   if (warp_id() == 0) {
     walk.start(p, (int)blockIdx.x, (int)gridDim.x);
-    if (tid == 0) p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) p.heads[blockIdx.x] = PagedHead{};
   }
   const int group = p.g;
   for (;;) {
@@ -420,11 +448,11 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           if (tx + 16 * c >= limit) s[i][c] = -INFINITY;
-          mx = fmaxf(mx, s[i][c]);
+          mx = max_nan(mx, s[i][c]);
         }
 #pragma unroll
-        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-        const float m_old = s_m[r], m_new = fmaxf(m_old, mx);
+        for (int w = 8; w > 0; w >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float m_old = s_m[r], m_new = max_nan(m_old, mx);
         const float base = m_new == -INFINITY ? 0.0f : m_new;  // a row that has seen no key yet
         float sum = 0.0f;
 #pragma unroll
@@ -477,16 +505,17 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
       const float m = s_m[r], l = s_l[r];
       const int fr = x.row0 + r;
       const long long at = (long long)(x.q0 + fr / group) * p.Hq + (long long)x.kvh * group + fr % group;
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const bool sees = paged_limit(p, x, fr) > 0;
+      const float inv = paged_inv(m, l);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const int d = tx * CV + 16 * (c - c % CV) + c % CV;
-        if (whole) stf((T*)p.out + at * D + d, o[i][c] * inv);
+        if (whole) stf((T*)p.out + at * D + d, sees ? o[i][c] * inv : 0.0f);
         else reinterpret_cast<float*>(paged_part(p, slot, d / 4, r))[d % 4] = o[i][c];
       }
       if (tx != 0) continue;
       if (!whole) p.part_ml[(long long)slot * p.rpi + r] = make_float2(m * 1.4426950408889634f, l);
-      else if (p.lse != nullptr) p.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
+      else if (p.lse != nullptr) p.lse[at] = fabsf(m) < INFINITY ? m + logf(l) : m;
     }
   }
 }
@@ -499,7 +528,7 @@ __global__ void __launch_bounds__(256) k_paged_attn_simt(const T* __restrict__ q
 constexpr int kPagedMostRuns = 320;  // of any attention kernel that leaves its joins to this one
 template <typename T>
 __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int runs) {
-  __shared__ int4 heads[kPagedMostRuns];
+  __shared__ PagedHead heads[kPagedMostRuns];
   __shared__ int first[kPagedMostRuns + 1];  // 32-row blocks of the items before
   pdl_launch_dependents();
   pdl_wait();
@@ -509,7 +538,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
   if (warp_id() == 0) {
     int sum = 0;
     for (int c0 = 0; c0 < runs; c0 += 32) {
-      const int blocks = c0 + lane < runs ? ((heads[c0 + lane].w & 0xffff) + 31) / 32 : 0;
+      const int blocks = c0 + lane < runs ? (heads[c0 + lane].rows + 31) / 32 : 0;
       int end = blocks;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -528,10 +557,10 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
     int c = 0;
     for (int step = 256; step > 0; step >>= 1)
       if (c + step < runs && first[c + step] <= block) c += step;  // the last item that starts at or before it
-    const int4 h = heads[c];
-    const int r = (block - first[c]) * 32 + lane, rows = h.w & 0xffff;
-    const PagedPieces pc{c, h.w >> 16};
-    if (r >= rows) continue;
+    const PagedHead h = heads[c];
+    const int r = (block - first[c]) * 32 + lane;
+    const PagedPieces pc{c, h.pieces};
+    if (r >= h.rows) continue;
     // one pass over the pieces with a running maximum, four pieces' loads at a time.  A piece without a
     // key of this row has left old values in its slot: read all the same, so that no load waits for
     // another, and passed over.
@@ -547,7 +576,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[i][q] = *paged_part(p, slot, c0 + q, r);
       }
-      const float m_new = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), mx);
+      const float m_new = max3_nan(max_nan(ml[0].x, ml[1].x), max_nan(ml[2].x, ml[3].x), mx);
       if (m_new == -INFINITY) continue;
       const float alpha = exp2f(mx - m_new);
       mx = m_new;
@@ -568,12 +597,13 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
         }
       }
     }
-    const int fr = h.z + r;
-    const long long at = (long long)(h.x + fr / p.g) * p.Hq + (long long)h.y * p.g + fr % p.g;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int fr = h.row0 + r;
+    const long long at = (long long)(h.q0 + fr / p.g) * p.Hq + (long long)h.kvh * p.g + fr % p.g;
+    const bool sees = (p.causal ? h.lim + fr / p.g : h.lim) > 0;
+    const float inv = paged_inv(mx, l);
     T* dst = (T*)p.out + at * p.D + 4 * c0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] *= inv;
+    for (int e = 0; e < 16; ++e) o[e] = sees ? o[e] * inv : 0.0f;
     if ((reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
       store8(dst, *reinterpret_cast<const float(*)[8]>(&o[0]));
       store8(dst + 8, *reinterpret_cast<const float(*)[8]>(&o[8]));
@@ -581,7 +611,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedParams p, int run
 #pragma unroll
       for (int e = 0; e < 16; ++e) stf(dst + e, o[e]);
     }
-    if (c0 == 0 && p.lse != nullptr) p.lse[at] = l > 0.0f ? (mx + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    if (c0 == 0 && p.lse != nullptr) p.lse[at] = paged_lse(mx, log2f(l));
   }
 }
 

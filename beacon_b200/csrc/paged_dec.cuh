@@ -52,8 +52,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+  v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return max_nan(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
@@ -160,15 +160,15 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
   auto store_row = [&](const PagedItem& x, int r, float m, float l, const float (&o)[CPL]) {
     const int fr = x.row0 + r;
     const long long at = (long long)(x.q0 + fr / p.g) * p.Hq + (long long)x.kvh * p.g + fr % p.g;
-    const bool none = m == -INFINITY;
-    const float inv = none ? 0.0f : 1.0f / l;
+    const bool sees = paged_limit(p, x, fr) > 0;
+    const float inv = paged_inv(m, l);
     uint32_t w[CPL / 2];
 #pragma unroll
-    for (int e = 0; e < CPL; e += 2) w[e / 2] = none ? 0u : pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+    for (int e = 0; e < CPL; e += 2) w[e / 2] = !sees ? 0u : pack_bf16x2(o[e] * inv, o[e + 1] * inv);
     uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at * D + CPL * lane);
     if constexpr (CPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
     else dst[0] = w[0];
-    if (lane == 0 && p.lse != nullptr) p.lse[at] = none ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+    if (lane == 0 && p.lse != nullptr) p.lse[at] = paged_lse(m, __log2f(l));
   };
 
   PagedItem x;
@@ -213,12 +213,12 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
 #pragma unroll
         for (int e = 0; e < 2 * NT; ++e) {
           v[e] = k0 + 8 * (e >> 1) + (e & 1) < lim[hf] ? sc[e >> 1][2 * hf + (e & 1)] * scale_log2 : -INFINITY;
-          mx = fmaxf(mx, v[e]);
+          mx = max_nan(mx, v[e]);
         }
         mx = quad_max(mx);
-        const float m_new = fmaxf(m[hf], mx);
-        // as long as the maximum grows by less than 2^8 the old one serves: O, l and P share it
-        const bool need = m_new > m[hf] + 8.0f;
+        const float m_new = max_nan(m[hf], mx);
+        // as long as the maximum grows by less than 2^8 the old one serves: O, l and P share it (a NaN is taken on)
+        const bool need = !(m_new <= m[hf] + 8.0f);
         if (__any_sync(0xffffffffu, need)) {
           const float alpha = need ? ex2_approx(m[hf] - m_new) : 1.0f;
           if (need) m[hf] = m_new;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
       if (r < rows) {  // row r: the warps' partial rows in warp order
         mbar_wait(&merge_full, merges & 1u, abort_flag, kSitePagedMerge);
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, mml[w * 8 + warp].x);
+        for (int w = 0; w < kDecWarps; ++w) mx = max_nan(mx, mml[w * 8 + warp].x);
         const float base = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
         for (int w = 0; w < kDecWarps; ++w) {
@@ -310,9 +310,9 @@ __global__ void __launch_bounds__(256, 1) k_paged_attn_dec(const __nv_bfloat16* 
       if (!paged_last_piece(p, pc, r)) continue;
       // lane i weighs piece i (of 32 at a time); the pieces' rows then load side by side
       mx = -INFINITY;
-      for (int i = lane; i < pc.n; i += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);
+      for (int i = lane; i < pc.n; i += 32) mx = max_nan(mx, __ldcg(&p.part_ml[pc.slot(i) * p.rpi + r]).x);
 #pragma unroll
-      for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      for (int w = 16; w > 0; w >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float base = mx == -INFINITY ? 0.0f : mx;
       lt = 0.0f;
 #pragma unroll

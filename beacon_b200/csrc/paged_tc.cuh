@@ -91,8 +91,8 @@ __device__ __forceinline__ int ptc_count(const PtcItem& x, int t) {
 // 2^a for a pair of arguments on the FMA pipe: a = n + f, f in [-0.5, 0.5], a quartic in f fitted to 2^f by
 // Lawson's iteration on the relative error (2.7e-6 in fp32), n added to the exponent.  The quartic, not
 // the cubic of the training forward, because lse is returned to 1e-5.  Arguments below -126, -inf
-// included, give less than 2^-125 instead of 0: masked keys add at most that to a row's sums, and a row
-// that sees no key is known by its maximum.
+// included, give less than 2^-125 instead of 0: masked keys add at most that to a row's sums.  NaN and
+// +inf are lost here; the row's maximum keeps them (paged_inv).
 __device__ __forceinline__ void exp2_poly4(float& r0, float& r1, float a0, float a1) {
   constexpr float kMagic = 12582912.0f;  // 1.5 x 2^23: adding it rounds to an integer
   a0 = fmaxf(a0, -126.0f);
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(384, 1)
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
         pdl_launch_dependents();
-        p.heads[blockIdx.x] = make_int4(0, 0, 0, 0);
+        p.heads[blockIdx.x] = PagedHead{};
       }
       PagedWalk<128, kPtcTile, kPtcDualTile> walk;
       walk.start(p, (int)blockIdx.x, (int)gridDim.x);
@@ -536,19 +536,20 @@ __global__ void __launch_bounds__(384, 1)
         float* xs = reinterpret_cast<float*>(xu);
         float m8[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) m8[u] = fmaxf(xs[u], xs[8 + u]);
+        for (int u = 0; u < 8; ++u) m8[u] = max_nan(xs[u], xs[8 + u]);
 #pragma unroll
         for (int c = 16; c < 128; c += 16)
 #pragma unroll
-          for (int u = 0; u < 8; ++u) m8[u] = fmax3(m8[u], xs[c + u], xs[c + 8 + u]);
-        const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) *
-                         tp.scale_log2;
-        const float m_new = fmaxf(m_used, mx);
+          for (int u = 0; u < 8; ++u) m8[u] = max3_nan(m8[u], xs[c + u], xs[c + 8 + u]);
+        const float mx =
+            max3_nan(max3_nan(m8[0], m8[1], m8[2]), max3_nan(m8[3], m8[4], m8[5]), max_nan(m8[6], m8[7])) *
+            tp.scale_log2;
+        const float m_new = max_nan(m_used, mx);
         if (i == 0) {
           m_used = m_new;
         } else {
-          // a row without a key so far has O = 0 and m = -inf: 2^(-inf) = 0 rescales it
-          const bool need = m_new > m_used + 8.0f;
+          // a row without a key so far has O = 0 and m = -inf: 2^(-inf) = 0 rescales it; a NaN is taken on
+          const bool need = !(m_new <= m_used + 8.0f);
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? ex2_approx(m_used - m_new) : 1.0f;
             if (need) {
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(384, 1)
         if (!ok) break;
         tc_fence_after();
         const float2 ml = dual_ml[(1 - t) * 128 + r];
-        const float mx = fmaxf(m_used, ml.x);
+        const float mx = max_nan(m_used, ml.x);
         const float base = mx == -INFINITY ? 0.0f : mx;
         const float w_own = ex2_approx(m_used - base), w_other = ex2_approx(ml.x - base);
         w_a = t == 0 ? w_own : w_other;
@@ -633,8 +634,9 @@ __global__ void __launch_bounds__(384, 1)
       const long long at = (long long)(x.tok0 + tok) * p.Hq + (long long)x.kvh * p.g + head;
       __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(p.out) + at * D;
       const bool out32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+      const bool none = lim <= 0;  // the row sees no key
       // stores 32 finished columns of the row, u inv
-      auto store_o = [&](int c, const uint32_t (&u)[32], float inv, bool none) {
+      auto store_o = [&](int c, const uint32_t (&u)[32], float inv) {
 #pragma unroll
         for (int e = 0; e < 32; e += 16) {
           uint32_t wv[8];
@@ -654,15 +656,14 @@ __global__ void __launch_bounds__(384, 1)
       const bool lse_row = p.lse != nullptr && !(x.dual && t == 1);
       if (x.slot < 0) {
         if (!has) continue;  // a tile B without rows
-        const bool none = m_used == -INFINITY;
-        const float inv = none ? 0.0f : 1.0f / l;
+        const float inv = paged_inv(m_used, l);
 #pragma unroll 1
         for (int c = c0; c < c1 && any_row; ++c) {
           uint32_t u[32];
           load_o(c, u);
-          if (row_ok) store_o(c, u, inv, none);
+          if (row_ok) store_o(c, u, inv);
         }
-        if (row_ok && lse_row) p.lse[at] = none ? -INFINITY : (m_used + __log2f(l)) * 0.69314718055994531f;
+        if (row_ok && lse_row) p.lse[at] = paged_lse(m_used, __log2f(l));
       } else if (any_row) {
         const int row = (x.dual ? 0 : t * tp.tpt * p.g) + r;  // row of the item
         // statistics of the row; B keeps its own copy of a dual item's, in rows that the item does not have
@@ -687,12 +688,12 @@ __global__ void __launch_bounds__(384, 1)
           const int mine = x.a > 0 ? 1 : 0;  // this piece is the item's first or second
           const long long that = x.pieces.slot(1 - mine);
           const float2 ml = row_ok ? __ldcg(&p.part_ml[that * p.rpi + ml_row]) : make_float2(-INFINITY, 0.0f);
-          const float mx = fmaxf(m_used, ml.x);
-          const bool none = mx == -INFINITY, read = row_ok && ml.x != -INFINITY;
-          const float base = none ? 0.0f : mx;
+          const float mx = max_nan(m_used, ml.x);
+          const bool read = row_ok && ml.x != -INFINITY;
+          const float base = mx == -INFINITY ? 0.0f : mx;
           const float w_mine = ex2_approx(m_used - base), w_that = ex2_approx(ml.x - base);
           const float lt = mine ? fmaf(l, w_mine, ml.y * w_that) : fmaf(ml.y, w_that, l * w_mine);
-          const float inv = none ? 0.0f : 1.0f / lt;
+          const float inv = paged_inv(mx, lt);
           const float4* src = paged_part(p, that, 8 * c0, row);
           float4 v[8];
 #pragma unroll
@@ -717,9 +718,9 @@ __global__ void __launch_bounds__(384, 1)
               for (int e = 0; e < 8; ++e)
                 v[e] = read ? __ldcg(src + (long long)(8 * (c + 1 - c0) + e) * p.rpi) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            if (row_ok) store_o(c, u, inv, none);
+            if (row_ok) store_o(c, u, inv);
           }
-          if (row_ok && lse_row) p.lse[at] = none ? -INFINITY : (mx + __log2f(lt)) * 0.69314718055994531f;
+          if (row_ok && lse_row) p.lse[at] = paged_lse(mx, __log2f(lt));
         }
         __syncwarp();
       }
