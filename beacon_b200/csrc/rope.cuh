@@ -698,6 +698,17 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
     if (w.kind != 2) ln.turn(p, pl.pos, c, s);
     cp_async_wait<kRopeStages - 1>();
     T* row = dqkv + t * p.ld_out + (long long)w.col * D;
+    if (pl.pos < 0 && w.kind != 2) {  // no position: zeros whatever dy and x hold, and nothing for the gains
+      const float none[8] = {};
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = w.h0 + u * HPW;
+        if (h >= w.count) continue;
+        store8(row + (long long)h * D + ln.e0, none);
+        store8(row + (long long)h * D + ln.e1, none);
+      }
+      continue;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h = w.h0 + u * HPW;
@@ -723,7 +734,7 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
         unraw(g0, ga);
         unraw(g1, gz);
         float inv = rsqrtf(ln.sum(dot8(xa, xa, xz, xz)) * (1.0f / D) + p.eps);
-        if (h >= w.count || pl.pos < 0) inv = 0.0f;  // no head, or no position: nothing is added
+        if (h >= w.count) inv = 0.0f;  // no head: nothing is added
         scale8(a, a, inv);  // dz / r
         scale8(z, z, inv);
         fma8(acc0, a, xa, acc0);
@@ -733,9 +744,6 @@ __global__ void __launch_bounds__(256, 2) k_qk_norm_rope_bwd_vec(T* __restrict__
         const float back = ln.sum(dot8(a, xa, z, xz)) * inv * inv * (-1.0f / D);
         fmaw8(a, xa, back, a);  // dx = e / r - x sum(e x / r) / (D r^2)
         fmaw8(z, xz, back, z);
-      } else if (pl.pos < 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = z[i] = 0.0f;
       }
       if (h >= w.count) continue;
       store8(row + (long long)h * D + ln.e0, a);
