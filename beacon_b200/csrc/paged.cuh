@@ -77,18 +77,22 @@ __device__ __forceinline__ int paged_tiles(const PagedParams& p, int i, int q_le
 __device__ __forceinline__ int paged_items(int q_len, int g, int rpi) {
   return (int)(((unsigned)q_len * (unsigned)g + (unsigned)rpi - 1u) / (unsigned)rpi);
 }
-// First token, new tokens and cached tokens of sequence s, held inside the tensors that they index.
-__device__ __forceinline__ void paged_lens(const PagedParams& p, int s, int& q0, int& q_len, int& kv) {
+// First token, new tokens and cached tokens of sequence s, held inside the tensors that they index; whether cu_q
+// does not decrease there.
+__device__ __forceinline__ bool paged_lens(const PagedParams& p, int s, int& q0, int& q_len, int& kv) {
   q0 = __ldg(p.pg.cu_q + s);
-  q_len = max(0, __ldg(p.pg.cu_q + s + 1) - q0);
+  int q1 = __ldg(p.pg.cu_q + s + 1);
   kv = max(0, __ldg(p.pg.kv_lens + s));
+  const bool rises = q1 >= q0;
   const long long most = (long long)p.pg.max_pages * p.pg.page_size;
-  if (q0 < 0 || (long long)q0 + q_len > p.tokens || kv > most) {
+  if (q0 < 0 || !rises || q1 > p.tokens || kv > most) {
     record_fault(kFaultIndex, kSitePagedLens);
-    q0 = max(q0, 0);
-    q_len = (int)max(0LL, min((long long)q_len, p.tokens - q0));
+    q0 = min(max(q0, 0), (int)p.tokens);
+    q1 = min(max(q1, q0), (int)p.tokens);
     kv = (int)min((long long)kv, most);
   }
+  q_len = q1 - q0;
+  return rises;
 }
 
 // A run, walked item by item by one warp (every lane holds the same state).  KT keys make a tile; W is its
@@ -104,10 +108,11 @@ struct PagedWalk {
     if constexpr (W == HW) return W;
     return q_len * p.g - i * p.rpi <= p.half_rows ? HW : W;
   }
-  __device__ __forceinline__ static int work(const PagedParams& p, int s) {  // of one KV head of sequence s
+  // Of one KV head of sequence s; falls: set where cu_q decreases.
+  __device__ __forceinline__ static int work(const PagedParams& p, int s, bool& falls) {
     if (s >= p.pg.seqs) return 0;
     int q0, q_len, kv;
-    paged_lens(p, s, q0, q_len, kv);
+    if (!paged_lens(p, s, q0, q_len, kv)) falls = true;
     const int n = paged_items(q_len, p.g, p.rpi);
     if (n == 0) return 0;
     int w = n * p.item_cost + weight(p, n - 1, q_len) * paged_tiles(p, n - 1, q_len, kv, KT);
@@ -119,10 +124,14 @@ struct PagedWalk {
   __device__ __forceinline__ void start(const PagedParams& p, int run, int runs) {
     const int lane = (int)lane_id();
     begin = end = pos = seq = kvh = item = q0 = q_len = kv = items = 0;  // an empty run is never walked
-    const int w0 = work(p, lane);
+    bool falls = false;
+    const int w0 = work(p, lane, falls);
     int total = w0;
 #pragma unroll 1
-    for (int s = lane + 32; s < p.pg.seqs; s += 32) total += work(p, s);
+    for (int s = lane + 32; s < p.pg.seqs; s += 32) total += work(p, s, falls);
+    // Sequences that overlap may hold more than p.tokens rows together, which the host's bound on the length of
+    // all work does not cover: such a call does nothing.
+    if (__any_sync(0xffffffffu, falls)) return;
     total = __reduce_add_sync(0xffffffffu, total) * p.Hkv;
     chunk = max(W > HW ? W : HW, (int)(((unsigned)total + (unsigned)runs - 1u) / (unsigned)runs));
     const int from = (int)min((unsigned)run * (unsigned)chunk, (unsigned)total);
@@ -130,7 +139,7 @@ struct PagedWalk {
     int at = from;
 #pragma unroll 1
     for (int s0 = 0; s0 < p.pg.seqs; s0 += 32) {
-      const int per_head = s0 == 0 ? w0 : work(p, s0 + lane);
+      const int per_head = s0 == 0 ? w0 : work(p, s0 + lane, falls);
       int sum = per_head * p.Hkv;  // inclusive prefix sum
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

@@ -46,7 +46,7 @@ struct RopeParams {
 
 enum : unsigned int {
   kSiteRopePosition = 0x601,  // a position outside the table, or before the sequence's start
-  kSiteRopePage = 0x602,      // a page index outside the cache, or a token past the page table
+  kSiteRopePage = 0x602,      // a page index outside the cache, a token past the page table, or a cu_q that decreases
 };
 
 // Number of i in [1, n] with cu[i] <= t (the sequence that owns token t; n: none does).
@@ -88,14 +88,17 @@ __device__ __forceinline__ TokenPlace token_place(const RopeParams& p, int t, To
     const PagedSeqs& g = p.pg;
     if (q.s < 0 || t < q.first || t >= q.end) {
       q.s = warp_owner(g.cu_q, g.seqs, t);
-      if (q.s >= g.seqs || t < __ldg(g.cu_q)) {
+      if (q.s < g.seqs) {
+        q.first = __ldg(g.cu_q + q.s);
+        q.end = __ldg(g.cu_q + q.s + 1);
+        q.kv = max(0, __ldg(g.kv_lens + q.s));
+      }
+      if (q.s >= g.seqs || t < q.first || t >= q.end) {
+        if (q.s < g.seqs && t >= q.end && lane_id() == 0) record_fault(kFaultIndex, kSiteRopePage);  // cu_q decreases
         q.s = -1;
         w.on = false;
         return w;
       }
-      q.first = __ldg(g.cu_q + q.s);
-      q.end = __ldg(g.cu_q + q.s + 1);
-      q.kv = __ldg(g.kv_lens + q.s);
     }
     const int s = q.s, at = q.kv - (q.end - t);
     w.pos = at;

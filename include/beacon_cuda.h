@@ -383,7 +383,8 @@ size_t beacon_qk_norm_rope_bwd_workspace_size(int64_t head_dim);
  * lives as long as its graph: the library's buffer is freed when a later call needs a larger one, so NULL
  * is refused with InvalidLaunchConfig on a stream that is being captured.  A page index outside the cache is not
  * followed (its tokens are not written, its keys and values read as zeros), and lengths that reach
- * past the tensors are cut; both record fault code 3.  Token rows that no sequence owns are ignored.
+ * past the tensors are cut; with a cu_q that decreases attention does nothing and the tokens that it
+ * gives no place are not written.  All record fault code 3.  Token rows that no sequence owns are ignored.
  *
  * qk_norm_rope_append: beacon_qk_norm_rope_fwd for new tokens, the queries written token-major
  * [tokens, q_heads, head_dim], keys and values into the pages.  Tokens rotate by their place j in the
