@@ -222,6 +222,8 @@ def _scratch(workspace, need, device):
     it for a graph that captures the call, where the caller gave none."""
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif not workspace.is_cuda or not workspace.is_contiguous():
+        raise InvalidLaunchConfig("the workspace must be a contiguous CUDA tensor")
     return workspace, workspace.numel() * workspace.element_size()
 
 
@@ -570,28 +572,34 @@ def llama_block_paged_fwd(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_do
     """llama_block_fwd for the new tokens x [T, d_model] of a batch of sequences with cached keys and values
     (tables as in qk_norm_rope_append): h = x + attn(rope(norm(rmsnorm(x) Wqkv)), cache) Wo;
     out = h + swiglu(rmsnorm(h)).  The new tokens' keys and values are written to the pages."""
-    seqs, *paging, Hkv, D, dtype = _paging("llama_block_paged_fwd", k_cache, v_cache, page_table, cu_q, kv_lens)
-    T, dm = x.shape
-    dt = _dtype(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_down, q_gain, k_gain)
+    what = "llama_block_paged_fwd"
+    if x.dim() != 2 or k_cache.dim() != 4 or w_gate.dim() != 2:
+        raise InvalidLaunchConfig(f"{what}: x [T, d_model], caches [pages, kv_heads, page_size, head_dim], w_gate [d_model, d_ff]")
+    (T, dm), Hkv, D, F = x.shape, k_cache.shape[1], k_cache.shape[3], w_gate.shape[1]
+    for name, t, shape in (("w_qkv", w_qkv, (dm, (heads + 2 * Hkv) * D)), ("w_o", w_o, (heads * D, dm)),
+                           ("w_gate", w_gate, (dm, F)), ("w_up", w_up, (dm, F)), ("w_down", w_down, (F, dm))):
+        if t.shape != shape:
+            raise InvalidLaunchConfig(f"{what}: {name} {tuple(t.shape)} is not {shape} (x {tuple(x.shape)}, {heads} + 2 x "
+                                      f"{Hkv} heads of {D}, d_ff {F})")
+    for name, t, n in (("attn_norm", attn_norm, dm), ("ffn_norm", ffn_norm, dm), ("q_gain", q_gain, D),
+                       ("k_gain", k_gain, D), ("out", out, T * dm)):
+        if t is not None and t.numel() != n:
+            raise InvalidLaunchConfig(f"{what}: {name} {tuple(t.shape)} does not hold {n} elements")
+    seqs, *paging, Hkv, D, dtype = _paging(what, k_cache, v_cache, page_table, cu_q, kv_lens)
+    dt = _dtype(x, attn_norm, w_qkv, w_o, ffn_norm, w_gate, w_up, w_down, q_gain, k_gain, out)
     if x.dtype is not dtype:
-        raise InvalidLaunchConfig(f"llama_block_paged_fwd: x of {x.dtype} beside caches of {dtype}")
-    if w_qkv.shape != (dm, (heads + 2 * Hkv) * D) or w_o.shape != (heads * D, dm):
-        raise InvalidLaunchConfig(f"llama_block_paged_fwd: w_qkv {tuple(w_qkv.shape)} and w_o {tuple(w_o.shape)} do not "
-                                  f"fit {heads} + 2 x {Hkv} heads of {D}")
-    for g in (q_gain, k_gain):
-        if g is not None and g.numel() != D:
-            raise InvalidLaunchConfig(f"llama_block_paged_fwd: gains must have {D} elements")
+        raise InvalidLaunchConfig(f"{what}: x of {x.dtype} beside caches of {dtype}")
     if table is not None and not (table.dtype is torch.float32 and table.dim() == 2 and table.is_cuda
                                   and table.is_contiguous()):
         raise InvalidLaunchConfig("llama_block_paged_fwd: the rotation table must be a contiguous float32 CUDA matrix")
     rows, rot = (0, 0) if table is None else table.shape
     if out is None:
         out = torch.empty_like(x)
-    workspace, wsb = _scratch(workspace, llama_block_paged_workspace_bytes(T, dm, heads, Hkv, D, w_gate.shape[1]), x.device)
+    workspace, wsb = _scratch(workspace, llama_block_paged_workspace_bytes(T, dm, heads, Hkv, D, F), x.device)
     check(_lib.lib().beacon_llama_block_paged_fwd(
         _p(out), _p(x), _p(attn_norm), _p(w_qkv), _p(q_gain), _p(k_gain), _p(w_o), _p(ffn_norm), _p(w_gate), _p(w_up),
         _p(w_down), _p(table), rows, rot, int(interleaved), _p(k_cache), _p(v_cache), _p(cu_q), _p(kv_lens),
-        _p(page_table), T, seqs, int(max_q or 0), *paging, dm, heads, Hkv, D, w_gate.shape[1], eps, dt,
+        _p(page_table), T, seqs, int(max_q or 0), *paging, dm, heads, Hkv, D, F, eps, dt,
         _p(workspace), wsb, _stream()))
     return out
 
