@@ -70,8 +70,8 @@ class KernelArgC(ctypes.Structure):
 
 
 def build(force: bool = False) -> str:
-    """Compile libbeacon_cuda.so in place with nvcc for sm_100a."""
-    cmd = ["make", "-s", "-C", CSRC]
+    """Compile libbeacon_cuda.so (nvcc, sm_100a) and beacon_front.so (the C++ compiler) in place."""
+    cmd = ["make", "-s", "-C", CSRC, "all", "front"]
     if force:
         cmd.insert(1, "-B")
     subprocess.run(cmd, check=True)
@@ -173,25 +173,45 @@ def lib():
 _front = None
 
 
+class _NoFront:
+    """Stands in for beacon_front where it cannot be loaded: it takes no operands, and ops makes each call itself."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def front():
     """beacon_front (csrc/front.cpp), bound to the library's entry points: the torch call path of the
-    operators that run once or twice per layer and token."""
+    operators that run once or twice per layer and token.  Without it, or with one built against another
+    torch, they run through ops' own checks and ctypes, some 10 us a call slower; a warning says so once."""
     global _front
     if _front is None:
-        import importlib.util
+        import warnings
 
-        import torch  # noqa: F401  (its libraries resolve the module's symbols)
-        if not os.path.exists(FRONT_PATH):
-            raise OSError(f"beacon_front.so not built at {FRONT_PATH}; run beacon_b200._lib.build()")
-        spec = importlib.util.spec_from_file_location("beacon_front", FRONT_PATH)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        mod.bind(*(ctypes.cast(getattr(lib(), n), _vp).value for n in (
-            "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd", "beacon_qk_norm_rope_append",
-            "beacon_paged_attention_fwd", "beacon_qk_norm_rope_bwd_workspace_size",
-            "beacon_paged_attention_workspace_size")))
-        _front = mod
+        lib()  # the library itself is not optional
+        try:
+            _front = _load_front()
+        except (OSError, ImportError, ValueError) as e:
+            warnings.warn(f"beacon_front.so is not used ({e}); build it with beacon_b200._lib.build()", RuntimeWarning,
+                          stacklevel=3)
+            _front = _NoFront()
     return _front
+
+
+def _load_front():
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries resolve the module's symbols)
+    if not os.path.exists(FRONT_PATH):
+        raise OSError(f"not built at {FRONT_PATH}")
+    spec = importlib.util.spec_from_file_location("beacon_front", FRONT_PATH)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind(*(ctypes.cast(getattr(lib(), n), _vp).value for n in (
+        "beacon_qk_norm_rope_fwd", "beacon_qk_norm_rope_bwd", "beacon_qk_norm_rope_append",
+        "beacon_paged_attention_fwd", "beacon_qk_norm_rope_bwd_workspace_size",
+        "beacon_paged_attention_workspace_size")))
+    return mod
 
 
 def last_error() -> str:
