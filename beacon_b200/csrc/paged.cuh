@@ -250,7 +250,8 @@ __device__ __forceinline__ PagedPieces paged_pieces(const PagedItem& x) { return
 // Pieces finished per split item (by its first run) and part of its rows.  The counters lie in the call's
 // workspace and k_paged_clear, launched ahead on the stream, zeroes them for every execution of the call,
 // replays of a captured one included: whatever the workspace held before, and whatever runs beside the
-// call with a workspace of its own, no count of another launch is ever seen.
+// call with a workspace of its own, no count of another launch is ever seen.  It costs 0.65 us of GPU time
+// beside a decode of 10 us, and 2.4 us of the host's.
 constexpr int kPagedMaxRuns = 160, kPagedParts = 16;
 __global__ void __launch_bounds__(256) k_paged_clear(uint4* __restrict__ done, int n) {
   pdl_launch_dependents();
@@ -317,7 +318,7 @@ __device__ __forceinline__ long long paged_key(const PagedSeqs& g, int seq, int 
 // of the item skips the arithmetic, so a decode step pays for its few rows only.  K and V of the next
 // tile are copied while this one is used (cp.async where rows are 16-byte aligned), its cache offsets
 // looked up one tile earlier still.  Bound: FFMA and shared-memory loads for full items (two 16-byte
-// loads per 16 FMA), HBM latency for short ones.
+// loads per 16 FMA), the serial phases of a run for short ones.
 // ---------------------------------------------------------------------------
 constexpr int kPagedSimtKt = 64, kPagedSimtRows = 64;
 template <int D>
@@ -328,8 +329,9 @@ constexpr size_t paged_simt_smem() {
 }
 
 // Exact form: products and sums in fp32 FFMA, 64 rows x 64 keys per step, 4 x 4 scores per thread, keys and
-// values copied a tile ahead.  Bound: FFMA issue for long work, the chain of a tile's two products for
-// short (8 sequences of 33-1500 keys, 1-40 new tokens, 8 / 4 heads of 64: 27 us).  Also takes bf16 calls that
+// values copied a tile ahead.  Bound: FFMA issue for long work.  For short work (8 sequences of 33-1500
+// keys, 1-40 new tokens, 8 / 4 heads of 64: 27 us) a run is one 64-key step, 2-3 us of FFMA; the rest is what
+// stands before and after it: finding the run, page lookups, copies, partial rows, the join's launch.  Also takes bf16 calls that
 // neither other kernel can: head_dim 16 and 32, and rows that are not 16-byte aligned.
 // ASYNC: T is float and the caches' rows are 16-byte aligned.
 template <typename T, int D, bool ASYNC>

@@ -24,12 +24,18 @@
 // of an item in two pieces are joined by the warp that finishes the second one; k_paged_join joins
 // those of items in more (one warp that reads 16 pieces took 45 us, the whole device a few).
 //
-// Bound: the softmax warps beside the tensor core.  2048 new tokens after 30720, 64/8 heads of 128: 1.70 ms =
-// 1.25 PFLOP/s, tensor pipe active 70% of the cycles.  A 256-row step of 128 keys takes ~3.0k cycles, of them
+// Bound: the softmax warps beside the tensor core.  2048 new tokens after 30720, 64/8 heads of 128: 1.73 ms =
+// 1.23 PFLOP/s on a GPU that comes from idle, 2.0 ms in a loop under the power cap; tensor pipe active 68% of
+// the cycles.  A 256-row step of 128 keys takes ~3.0k cycles, of them
 // ~1.75k in softmax and ~1.2k waiting for the S that was issued behind the other tile's PV.  Short items pay
 // ~7.5k cycles for their start and end (rows stored from registers, first softmax of both tiles at once):
-// 16 sequences of 1-512 new tokens after 100-7500, 32/8 heads, 103 us against 45 us of FLOPs.  Their code is
-// fetched anew at each item's end: unrolled by chunk it was slower (106 us).
+// 16 sequences of 1-512 new tokens after 100-7500, 32/8 heads, 103-106 us from idle and 118 in a loop of calls,
+// against 45 us of FLOPs.  Tiles, starts and ends, splits, the join and the launch at these costs make 80 to 85
+// of them; where the rest goes has not been measured.  An item's end is fetched anew each time:
+// unrolled by chunk it was slower (106 us against 103).
+//
+// P is rounded to bf16 because the operands of its product are of one type, the cached values': at most 2^-9
+// of each weight; the row's sum l keeps the unrounded ones.
 //
 // TMEM: S_A [0,128), S_B [128,256), O_A [256,256+D), O_B [256+D,256+2D).
 #pragma once
@@ -69,7 +75,8 @@ enum : unsigned int {
 
 constexpr int kPtcItems = 4;  // items published ahead
 // Time of a key tile, of one of a dual item, and of an item's start and end (clock counts of every CTA of a
-// launch over 16 sequences of 1-512 new tokens, fitted: 3390, 2330 and 7550 cycles).
+// launch over 16 sequences of 1-512 new tokens, heads of 128, fitted: 3390, 2330 and 7550 cycles).  Heads of 64
+// take the same weights, which were not fitted there: the same sequences 95 us against a floor of 22.
 constexpr int kPtcTile = 3, kPtcDualTile = 2, kPtcItemCost = 7;
 struct PtcItem {
   int valid;

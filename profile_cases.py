@@ -10,6 +10,13 @@
     python profile_cases.py residual_add | cast_f32_bf16 | dropout_fwd   (16384 x 4096 elements)
     python profile_cases.py block          (pre-norm block forward, batch 4 x seq 2048, d_model 4096)
     python profile_cases.py block_folded   (the same with both RMSNorms folded into the GEMMs)
+    python profile_cases.py rope_fwd       (8192 tokens of 32 + 32 + 32 heads of 128, bf16)
+    python profile_cases.py rope_bwd       (32768 tokens of 32 / 8 heads of 128, bf16)
+    python profile_cases.py rope_append    (6 prompts of 311-4096 tokens, 64 / 8 heads, into pages of 64)
+    python profile_cases.py paged_decode   (64 sequences of 500-8192 keys, one new token each, 32 / 8 heads, pages of 16)
+    python profile_cases.py paged_chunk    (2048 new tokens after 30720, 64 / 8 heads, pages of 128)
+    python profile_cases.py paged_mixed    (16 sequences of 1-512 new tokens after 100-7500, 32 / 8 heads, pages of 16)
+    python profile_cases.py paged_block    (a block step: --tokens new tokens, one a sequence, after 1000 each)
 
 Each case runs `--warmup` untimed launches and then `--iters` launches timed with
 CUDA events, printing the per-launch time and TFLOP/s (algorithmic FLOPs: causal
@@ -21,6 +28,8 @@ backward reads x and dy and writes dx (3 * tokens * width * 2 B) plus the statis
 read, timed over the whole call (row kernel and the two column sums).  The elementwise
 cases count their operands once: residual add and dropout 3 x 2 B per element (two bf16
 tensors in and one out, or one in and out plus the mask), the f32 -> bf16 cast 4 + 2 B.
+The rotation cases print GB/s of their rows read and written, the cache cases the time of the whole call
+(with the kernels that clear its counters and join split work) and the rate of its keys and values or products.
 Sizes default to
 a case larger than the 126 MB L2 but a few hundred MB on the device, the size an
 ncu capture of a single launch (-k <kernel> -s <warmup launches> -c 1) should use.
@@ -40,7 +49,8 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["attn_fwd", "attn_bwd", "attn_bwd_recompute", "gemm", "gemm_fp8", "swiglu_bwd",
                                      "swiglu_fwd", "block", "block_folded", "residual_add", "cast_f32_bf16",
-                                     "dropout_fwd",
+                                     "dropout_fwd", "rope_fwd", "rope_bwd", "rope_append", "paged_decode",
+                                     "paged_chunk", "paged_mixed", "paged_block",
                                      "layernorm_fwd", "layernorm_bwd", "rmsnorm_fwd", "rmsnorm_bwd"])
     ap.add_argument("--tokens", type=int, default=16384)
     ap.add_argument("--width", type=int, default=4096)
@@ -64,6 +74,8 @@ def main(argv=None):
     dev = torch.device("cuda", 0)
     if a.case.startswith(("layernorm", "rmsnorm", "residual", "cast", "dropout")):
         return _hbm_case(a, torch, ops, dev)
+    if a.case.startswith(("rope", "paged")):
+        return _cache_case(a, torch, ops, dev)
     if a.case.startswith("attn"):
         H, S, D = a.heads, a.seq, a.dim
         Hkv = a.kv_heads or H
@@ -192,6 +204,74 @@ def _hbm_case(a, torch, ops, dev):
     ms = e0.elapsed_time(e1) / a.iters
     print(f"{a.case}: tokens {T} width {W} {ms:.4f} ms/call {nbytes / (ms * 1e-3) / 1e9:.0f} GB/s algorithmic",
           flush=True)
+    ops.device_status(0)
+    return 0
+
+
+def _cache_case(a, torch, ops, dev):
+    """Position rotation, append and attention over a paged cache, heads of 128, bf16."""
+    D, bf = 128, torch.bfloat16
+    gen = torch.Generator(device=dev).manual_seed(0)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device=dev).to(bf)  # noqa: E731
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    gq, gk = rnd(D), rnd(D)
+    flops = nbytes = 0.0
+    if a.case == "rope_fwd":
+        T, H, K = 8192, 32, 32
+        x, table = rnd(T, (H + 2 * K) * D), ops.rope_table(2048, D)
+        fn, nbytes = (lambda: ops.qk_norm_rope_fwd(x, gq, gk, table, 4, T // 4, H, K)), 2.0 * x.numel() * 2
+    elif a.case == "rope_bwd":
+        T, H, K = 32768, 32, 8
+        x, table = rnd(T, (H + 2 * K) * D), ops.rope_table(4096, D)
+        dy = [rnd(8, n, T // 8, D) for n in (H, K, K)]
+        fn = lambda: ops.qk_norm_rope_bwd(*dy, x, gq, gk, table)  # noqa: E731
+        nbytes = 2.0 * (2 * x.numel() + T * (H + K) * D)
+    else:
+        spread = lambda lo, hi, n: [round(lo * (hi / lo) ** (i / max(n - 1, 1))) for i in range(n)]  # noqa: E731
+        q, before, H, K, page = {
+            "rope_append": (spread(311, 4096, 6), [0] * 6, 64, 8, 64),
+            "paged_decode": ([1] * 64, spread(500, 8192, 64), 32, 8, 16),
+            "paged_chunk": ([2048], [30720], 64, 8, 128),
+            "paged_mixed": (spread(1, 512, 16), [spread(100, 7500, 16)[(7 * i + 4) % 16] for i in range(16)], 32, 8, 16),
+            "paged_block": ([1] * min(a.tokens, 512), [1000] * min(a.tokens, 512), 32, 8, 16),
+        }[a.case]
+        kv = [m + n for m, n in zip(q, before)]
+        need = [-(-n // page) for n in kv]
+        order = torch.randperm(sum(need), generator=gen, device=dev).to(torch.int32)
+        pt = torch.zeros(len(q), max(need), dtype=torch.int32, device=dev)
+        for s, at in enumerate(torch.tensor([0] + need).cumsum(0)[:-1].tolist()):
+            pt[s, :need[s]] = order[at:at + need[s]]
+        T, cu, lens = sum(q), i32([0] + torch.tensor(q).cumsum(0).tolist()), i32(kv)
+        kc, vc = rnd(sum(need), K, page, D), rnd(sum(need), K, page, D)
+        table = ops.rope_table(max(kv), D)
+        if a.case == "rope_append":
+            x = rnd(T, (H + 2 * K) * D)
+            fn, nbytes = (lambda: ops.qk_norm_rope_append(x, gq, gk, table, kc, vc, pt, cu, lens, H)), 4.0 * x.numel()
+        elif a.case == "paged_block":
+            dm, F = a.width, 14336
+            w = lambda r, c: (torch.randn(r, c, generator=gen, device=dev) * 0.02).to(bf)  # noqa: E731
+            x, n1, n2 = rnd(T, dm), 1 + 0.1 * rnd(dm), 1 + 0.1 * rnd(dm)
+            wqkv, wo, wg, wu, wd = w(dm, (H + 2 * K) * D), w(H * D, dm), w(dm, F), w(dm, F), w(F, dm)
+            fn = lambda: ops.llama_block_paged_fwd(x, n1, wqkv, wo, n2, wg, wu, wd, kc, vc, pt, cu, lens, H,  # noqa: E731
+                                                   table=table, q_gain=gq, k_gain=gk, max_q=1)
+            nbytes = 2.0 * (wqkv.numel() + wo.numel() + 3 * wg.numel()) + 4.0 * sum(kv) * K * D
+        else:
+            qt = rnd(T, H, D)
+            fn = lambda: ops.paged_attention(qt, kc, vc, pt, cu, lens, max_q=max(q))  # noqa: E731
+            seen = sum(m * (n - m) + m * (m + 1) / 2 for m, n in zip(q, kv))
+            flops, nbytes = 4.0 * D * H * seen, 4.0 * sum(kv) * K * D + 4.0 * T * H * D
+    for _ in range(a.warmup):
+        fn()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    for _ in range(a.iters):
+        fn()
+    e1.record()
+    torch.cuda.synchronize()
+    ms = e0.elapsed_time(e1) / a.iters
+    print(f"{a.case}: {ms:.4f} ms/call {nbytes / (ms * 1e-3) / 1e9:.0f} GB/s algorithmic"
+          + (f" {flops / (ms * 1e-3) / 1e12:.0f} TFLOP/s" if flops else ""), flush=True)
     ops.device_status(0)
     return 0
 
